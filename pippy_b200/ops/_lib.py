@@ -34,8 +34,12 @@ SIGNATURES = {
     "pb_accum_bf16_into_f32": "pplp",
     "pb_adamw": "ppppplfffffifip",
     "pb_colsum_bf16": "pplilp",
+    "pb_dropout": "ppp" "l" "p" "ll" "ip",
     "pb_embed_bwd": "pppplii" "lp",
     "pb_embed_fwd": "pppplii" "lp",
+    "pb_embed_scaled_fwd": "ppppp" "lii" "lif" "pp",
+    "pb_embed_sorted_bwd": "ppppp" "liiii" "fi" "pp",
+    "pb_embed_sorted_scratch": "lii",
     "pb_flash_bwd": "p" * 10 + "iiiii" "llllll" "fipp",
     "pb_flash_fwd": "ppppp" "iiiii" "llll" "fipp",
     "pb_gelu_bwd": "ppplp",
@@ -43,6 +47,10 @@ SIGNATURES = {
     "pb_norm_bwd_res": "p" * 11 + "ip" "iiii" "p",
     "pb_norm_bwd_scratch_floats": "ii",
     "pb_norm_fwd": "p" * 6 + "iifip",
+    "pb_packed_attention_bwd": "p" * 12 + "i" "ppi" "liii" "llllll" "fipp",
+    "pb_packed_attention_fwd": "p" * 7 + "i" "liii" "llll" "fipp",
+    "pb_packed_layout": "piii" "ppp" "ipi" "ppp",
+    "pb_packed_rope": "plpl" "ppp" "liii" "pp",
     "pb_rope": "ppp" "liii" "lfp",
     "pb_scale_bf16": "pplp",
     "pb_set_gemm_group_m": "i",
@@ -73,6 +81,7 @@ def lib() -> ctypes.CDLL:
         handle = ctypes.CDLL(LIB_PATH)
         handle.pb_launch_count.restype = c_ll
         handle.pb_last_cuda_error.restype = ctypes.c_char_p
+        handle.pb_embed_sorted_scratch.restype = c_ll
         for name, types in SIGNATURES.items():
             getattr(handle, name).argtypes = [_TYPES[t] for t in types]
         _LIB = handle
@@ -133,7 +142,9 @@ def check_device_errors() -> None:
         if code != 0:
             w.zero_()
             raise KernelError(f"device {idx}: kernel error code {code} (1 = bounded wait ran out, 3 = peer wait ran out, "
-                              "4 = MoE receive buffer overflow, 5 = index out of range in a bounds-checking build)")
+                              "4 = MoE receive buffer overflow, 5 = index out of range (checked always by the packed-document and "
+                              "scaled-embedding kernels, elsewhere in a bounds-checking build), 6 = document lengths that are "
+                              "negative or exceed their row)")
 
 
 def check(rc: int, what: str) -> None:

@@ -12,8 +12,9 @@ run.
 """
 from __future__ import annotations
 
+import contextlib
 import math
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -26,6 +27,19 @@ from .gemm import ACT_GELU_TANH, ACT_NONE, gemm
 def _use_kernels(*tensors: torch.Tensor) -> bool:
     t = tensors[0]
     return t.is_cuda and t.dtype == torch.bfloat16
+
+
+def _on_device_of(t: torch.Tensor):
+    """Launches go to the current device's stream: makes ``t``'s device the current one where it is not."""
+    if not t.is_cuda or t.device.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and starting on a 16-byte boundary, as kernels with 16-byte accesses need it."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 _SM_COUNT = {}
@@ -559,14 +573,383 @@ class _EmbeddingFn(torch.autograd.Function):
         return None, None, None, None
 
 
-def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None):
-    """``wte[ids] (+ wpe[position])`` flattened to ``[B*S, H]``; position of token t is ``t % seq_len``."""
+class _SortedEmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, wte, wpe, positions, S: int, scale: float):
+        T, H = ids.numel(), wte.shape[1]
+        table, ptable = _aligned(wte.detach()), None if wpe is None else _aligned(wpe.detach())
+        out = torch.empty(T, H, device=wte.device, dtype=wte.dtype)
+        with _on_device_of(wte):
+            _lib.check(
+                _lib.lib().pb_embed_scaled_fwd(_lib.addr(ids), _lib.addr(table), _lib.addr(ptable),
+                                               _lib.addr(positions), _lib.addr(out), T, H, S, wte.shape[0],
+                                               0 if wpe is None else wpe.shape[0], scale, _lib.err_addr(wte.device),
+                                               _lib.stream_addr()),
+                "pb_embed_scaled_fwd",
+            )
+        ctx.save_for_backward(ids, positions)
+        wte._pb_direct_grad = True
+        if wpe is not None:
+            wpe._pb_direct_grad = True
+        ctx.params = (wte, wpe)  # not saved tensors: see _LinearFn.forward
+        ctx.cfg = (S, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        ids, positions = ctx.saved_tensors
+        wte, wpe = ctx.params
+        S, scale = ctx.cfg
+        d2 = _aligned(dout)
+        _run_or_defer(lambda: _embed_sorted_wgrad(ids, positions, d2, wte, wpe, S, scale))
+        return None, None, None, None, None, None
+
+
+def _embed_sorted_wgrad(ids, positions, dout, wte, wpe, S, scale):
+    T, H = dout.shape
+    params = [p for p in (wte, wpe) if p is not None and p.requires_grad]
+
+    def has_buffer(p):
+        mg = getattr(p, "main_grad", None)
+        return mg is not None and mg.dtype == torch.float32 and mg.is_contiguous() and mg.data_ptr() % 16 == 0
+
+    # the kernel adds to the parameters' fp32 buffers, or it writes gradients whole, in the parameters' type
+    direct = all(has_buffer(p) for p in params)
+    grads = [p.main_grad if direct else torch.empty(p.shape, dtype=p.dtype, device=p.device) for p in params]
+    where = {id(p): _lib.addr(g) for p, g in zip(params, grads)}
+    lib = _lib.lib()
+    scratch = torch.empty(lib.pb_embed_sorted_scratch(T, H, len(params)), dtype=torch.uint8, device=dout.device)
+    with _on_device_of(dout):
+        _lib.check(
+            lib.pb_embed_sorted_bwd(_lib.addr(ids), _lib.addr(positions), _lib.addr(dout), where.get(id(wte)),
+                                    where.get(id(wpe)), T, H, S, wte.shape[0], 0 if wpe is None else wpe.shape[0],
+                                    scale, int(not direct), _lib.addr(scratch), _lib.stream_addr()),
+            "pb_embed_sorted_bwd",
+        )
+        if not direct:
+            for p, g in zip(params, grads):
+                if getattr(p, "main_grad", None) is None and p.grad is None:
+                    p.grad = g
+                else:
+                    _accumulate_param_grad(p, g)
+
+
+def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 1.0,
+              positions: Optional[torch.Tensor] = None, sorted_grad: bool = False):
+    """``scale * wte[ids] (+ wpe[position])`` flattened to ``[B*S, H]``; position of token t is ``t % seq_len``, or
+    ``positions[t]`` where given (a :class:`PackedLayout`'s, -1 adds nothing).
+
+    The tables' gradients are fp32 scatter-adds, whose order changes from run to run, unless ``sorted_grad`` is set:
+    then, and always with a ``scale`` or ``positions``, tokens are sorted first and the rows of a token added in their
+    order, the same bits on every run.  On that path ids outside ``wte`` and positions beyond ``wpe`` give zeros and
+    set the device error word (:func:`pippy_b200.ops._lib.check_device_errors`)."""
     S = ids.shape[-1] if seq_len is None else seq_len
+    plain = scale == 1.0 and positions is None
+    if positions is not None:
+        if wpe is None:
+            raise ValueError("positions were given without a table of positions")
+        if positions.numel() != ids.numel() or positions.device != ids.device or positions.is_floating_point():
+            raise ValueError(f"positions: one integer for each of {ids.numel()} ids, on their device; got "
+                             f"{tuple(positions.shape)} {positions.dtype} on {positions.device}")
     if wte.is_cuda and wte.dtype == torch.bfloat16:
-        # autograd only tracks the op if some input requires grad; tie it to the table
-        return _EmbeddingFn.apply(ids, wte, wpe, S)
-    out = F.embedding(ids.reshape(-1), wte)
+        if plain and not sorted_grad:
+            # autograd only tracks the op if some input requires grad; tie it to the table
+            return _EmbeddingFn.apply(ids, wte, wpe, S)
+        if ids.device != wte.device or ids.is_floating_point():
+            raise ValueError(f"ids: integers on {wte.device}, got {ids.dtype} on {ids.device}")
+        if wte.dim() != 2 or wte.shape[1] % 8 or (wpe is not None and (
+                wpe.shape[1:] != wte.shape[1:] or wpe.dtype != wte.dtype or wpe.device != wte.device)):
+            raise ValueError("tables: [rows, H] of one type on one device, H a multiple of 8")
+        if positions is not None:
+            positions = positions.reshape(-1).to(torch.int32).contiguous()
+        return _SortedEmbeddingFn.apply(ids.reshape(-1).long().contiguous(), wte, wpe, positions, S, float(scale))
+    if plain:
+        out = F.embedding(ids.reshape(-1), wte)
+        if wpe is not None:
+            pos = torch.arange(ids.numel(), device=ids.device) % S
+            out = out + F.embedding(pos, wpe)
+        return out
+    wide = torch.promote_types(wte.dtype, torch.float32)
+    out = F.embedding(ids.reshape(-1), wte).to(wide) * scale
     if wpe is not None:
-        pos = torch.arange(ids.numel(), device=ids.device) % S
-        out = out + F.embedding(pos, wpe)
-    return out
+        pos = (torch.arange(ids.numel(), device=ids.device) % S) if positions is None else positions.reshape(-1).long()
+        out = out + torch.where((pos >= 0).unsqueeze(1), F.embedding(pos.clamp(min=0), wpe).to(wide), 0.0)
+    return out.to(wte.dtype)
+
+
+# ------------------------------------------------------------------------------------------------
+# packed documents
+# ------------------------------------------------------------------------------------------------
+class PackedLayout:
+    """Where the documents of a packed batch lie (:func:`packed_layout`).  One layout serves every layer of a batch, forward
+    and backward.
+
+    ``positions``: int32 ``[rows * tokens_per_row]``, each token's place in its document, -1 in padding."""
+
+    def __init__(self, lengths: torch.Tensor, tokens_per_row: int, positions: torch.Tensor):
+        self.lengths, self.tokens_per_row, self.positions = lengths, tokens_per_row, positions
+        self.rows = lengths.shape[0]
+        self.device = lengths.device
+        # kernel path: tile tables by rows per tile, the most entries they can have, and their used lengths
+        self.tiles: dict = {}
+        self.max_tiles: dict = {}
+        self.counts: dict = {}
+
+    @property
+    def total(self) -> int:
+        return self.rows * self.tokens_per_row
+
+
+def packed_layout(lengths: torch.Tensor, tokens_per_row: int) -> PackedLayout:
+    """The layout of rows of ``tokens_per_row`` tokens that hold documents one after the other: ``lengths`` is an integer
+    tensor ``[rows, documents]`` (or ``[documents]`` for one row); a length may be 0 (rows with fewer documents), and what a
+    row has left behind its last document is padding.
+
+    On the GPU this is one kernel: the lengths stay on the device and nothing waits for them.  Lengths that are negative or
+    exceed their row are cut to what fits and set the device error word
+    (:func:`pippy_b200.ops._lib.check_device_errors`); on the CPU they raise."""
+    if lengths.dim() == 1:
+        lengths = lengths.unsqueeze(0)
+    if lengths.dim() != 2 or lengths.shape[0] < 1 or lengths.is_floating_point() or lengths.is_complex() or \
+            lengths.dtype == torch.bool:
+        raise ValueError(f"lengths: integers [rows, documents], got {tuple(lengths.shape)} {lengths.dtype}")
+    rows, docs = lengths.shape
+    S = int(tokens_per_row)
+    if S < 1 or rows * S >= 2 ** 31 or rows * (docs + 1) >= 2 ** 31:
+        raise ValueError(f"{rows} rows of {S} tokens with {docs} documents each: between 1 and 2^31 - 1 of both")
+    if not lengths.is_cuda:
+        if docs and (bool((lengths < 0).any()) or int(lengths.long().sum(1).max()) > S):
+            raise ValueError(f"document lengths are negative or exceed the row of {S} tokens")
+        ends = lengths.long().cumsum(1)
+        t = torch.arange(S).expand(rows, S).contiguous()
+        positions = torch.full((rows, S), -1, dtype=torch.int32)
+        if docs:
+            doc = torch.searchsorted(ends, t, right=True)
+            starts = torch.cat([torch.zeros_like(ends[:, :1]), ends], 1)
+            positions = torch.where(t < ends[:, -1:], t - starts.gather(1, doc), -1).int()
+        return PackedLayout(lengths, S, positions.reshape(-1))
+    with _on_device_of(lengths):
+        # lengths beyond 32 bits would wrap to ones that seem to fit
+        given = (lengths if lengths.dtype == torch.int32 else lengths.clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
+        segments = rows * (docs + 1)
+        most = {n: rows * S // n + min(segments, rows * S) for n in (128, 256)}
+        # one buffer, every part on a 16-byte boundary: tiles of 4 ints, then segments, counts, positions
+        ints = 4 * (most[128] + most[256]), (2 * segments + 3) // 4 * 4, 4
+        buf = torch.empty(sum(ints) + rows * S, dtype=torch.int32, device=lengths.device)
+        tiles, segs, counts, positions = buf.split([*ints, rows * S])
+        layout = PackedLayout(given, S, positions)
+        layout.tiles = {128: tiles[: 4 * most[128]], 256: tiles[4 * most[128]:]}
+        layout.max_tiles, layout.counts = most, {128: counts[:1], 256: counts[1:2]}
+        _lib.check(
+            _lib.lib().pb_packed_layout(_lib.addr(given), rows, docs, S, _lib.addr(positions), _lib.addr(segs),
+                                        _lib.addr(layout.tiles[128]), most[128], _lib.addr(layout.tiles[256]), most[256],
+                                        _lib.addr(counts), _lib.err_addr(lengths.device), _lib.stream_addr()),
+            "pb_packed_layout",
+        )
+    return layout
+
+
+class _PackedAttentionFn(torch.autograd.Function):
+    """As :class:`_RopeAttentionFn`, over documents.  Without ``inplace`` the rotated q and k are a tensor of their own and
+    ``qkv`` stays as it is; its v columns are read in place either way."""
+
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, layout, Hq, Hkv, D, scale, causal, inplace):
+        T, nq, nk = layout.total, Hq * D, Hkv * D
+        lib, err = _lib.lib(), _lib.err_addr(qkv.device)
+        with _on_device_of(qkv):
+            qk = qkv
+            if cos is not None:
+                if not inplace:
+                    qk = torch.empty(T, nq + nk, device=qkv.device, dtype=qkv.dtype)
+                _lib.check(
+                    lib.pb_packed_rope(_lib.addr(qkv), qkv.stride(0), _lib.addr(qk), qk.stride(0), _lib.addr(cos),
+                                       _lib.addr(sin), _lib.addr(layout.positions), T, Hq + Hkv, D, cos.shape[0], err,
+                                       _lib.stream_addr()),
+                    "pb_packed_rope",
+                )
+                if inplace:
+                    torch.autograd.graph.increment_version(qkv)
+            q, k, v = qk[:, :nq], qk[:, nq : nq + nk], qkv[:, nq + nk :]
+            o = torch.empty(T, nq, device=qkv.device, dtype=qkv.dtype)
+            lse = torch.empty(Hq, T, device=qkv.device, dtype=torch.float32)
+            _lib.check(
+                lib.pb_packed_attention_fwd(_lib.addr(q), _lib.addr(k), _lib.addr(v), _lib.addr(o), _lib.addr(lse),
+                                            _lib.addr(layout.tiles[256]), _lib.addr(layout.counts[256]),
+                                            layout.max_tiles[256], T, Hq, Hkv, D, qk.stride(0), qk.stride(0),
+                                            qkv.stride(0), o.stride(0), scale, int(causal), err, _lib.stream_addr()),
+                "pb_packed_attention_fwd",
+            )
+        ctx.save_for_backward(qkv, qk, o, lse, cos, sin)
+        ctx.layout = layout
+        ctx.cfg = (Hq, Hkv, D, scale, causal)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        qkv, qk, o, lse, cos, sin = ctx.saved_tensors
+        layout = ctx.layout
+        Hq, Hkv, D, scale, causal = ctx.cfg
+        T, nq, nk = layout.total, Hq * D, Hkv * D
+        with _on_device_of(qkv):
+            do = _aligned(do)
+            q, k, v = qk[:, :nq], qk[:, nq : nq + nk], qkv[:, nq + nk :]
+            dqkv = torch.empty(T, nq + 2 * nk, device=qkv.device, dtype=qkv.dtype)
+            dq, dk, dv = dqkv[:, :nq], dqkv[:, nq : nq + nk], dqkv[:, nq + nk :]
+            delta = torch.empty(Hq, T, device=qkv.device, dtype=torch.float32)
+            _lib.check(
+                _lib.lib().pb_packed_attention_bwd(
+                    _lib.addr(do), _lib.addr(q), _lib.addr(k), _lib.addr(v), _lib.addr(o), _lib.addr(lse),
+                    _lib.addr(delta), _lib.addr(dq), _lib.addr(dk), _lib.addr(dv), _lib.addr(cos), _lib.addr(sin),
+                    0 if cos is None else cos.shape[0], _lib.addr(layout.tiles[128]), _lib.addr(layout.counts[128]),
+                    layout.max_tiles[128], T, Hq, Hkv, D, qk.stride(0), qk.stride(0), qkv.stride(0), o.stride(0),
+                    do.stride(0), dqkv.stride(0), scale, int(causal), _lib.err_addr(qkv.device), _lib.stream_addr()),
+                "pb_packed_attention_bwd",
+            )
+        return (dqkv,) + (None,) * 9
+
+
+def packed_attention(qkv, cos, sin, layout: PackedLayout, Hq: int, Hkv: int, D: int, scale: Optional[float] = None,
+                     causal: bool = True, inplace: bool = False):
+    """Self-attention inside each document of a packed batch: ``qkv`` is ``[layout.total, (Hq + 2*Hkv) * D]`` (q heads, then k
+    heads, then v heads), the result ``[layout.total, Hq * D]``.  Tokens see the tokens of their own document, with
+    ``causal`` those up to themselves; padding rows give zeros, in the result and in the gradient, whatever they hold.
+    Heads of q share the k and v heads in groups of ``Hq // Hkv``.
+
+    ``cos`` / ``sin`` (fp32 ``[positions, D / 2]``, see :func:`rope_tables`) rotate q and k by the position inside the
+    document; their rows have to reach the longest document (on the kernel path longer ones set the device error word and
+    stay unrotated from there on, on the CPU they raise).  With ``inplace`` the rotation overwrites the q and k columns
+    of ``qkv`` (its version counter is bumped), which saves a tensor of their size; without rotation it means nothing.
+
+    Kernel path (CUDA bf16): D is 64 or 128, no atomics, the same bits on every run."""
+    scale = (1.0 / math.sqrt(D)) if scale is None else float(scale)
+    if Hq < 1 or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads evenly")
+    if qkv.dim() != 2 or qkv.shape[0] != layout.total or qkv.shape[1] != (Hq + 2 * Hkv) * D:
+        raise ValueError(f"qkv: [{layout.total}, {(Hq + 2 * Hkv) * D}] for this layout and these heads, got "
+                         f"{tuple(qkv.shape)}")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale has to be positive and finite, got {scale}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    for t in () if cos is None else (cos, sin):
+        if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != D // 2 or t.dtype != torch.float32 or \
+                t.device != qkv.device:
+            raise ValueError(f"cos / sin: fp32 [positions, {D // 2}] on {qkv.device}, got {tuple(t.shape)} {t.dtype} on "
+                             f"{t.device}")
+    if layout.device != qkv.device:
+        raise ValueError(f"the layout is on {layout.device}, qkv on {qkv.device}")
+    if _use_kernels(qkv):
+        if D not in (64, 128):
+            raise ValueError(f"the kernels have head sizes 64 and 128, got {D}")
+        if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1] or qkv.data_ptr() % 16:
+            if inplace and cos is not None:
+                raise ValueError("inplace needs rows of unit stride that start on 16-byte boundaries")
+            qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
+        if cos is not None:
+            cos, sin = _aligned(cos), _aligned(sin)
+        return _PackedAttentionFn.apply(qkv, cos, sin, layout, Hq, Hkv, D, scale, causal, inplace)
+    rows, S = layout.rows, layout.tokens_per_row
+    pos = layout.positions.view(rows, S).long()
+    wide = torch.promote_types(qkv.dtype, torch.float32)
+    q, k, v = (t.reshape(rows, S, -1, D).transpose(1, 2).to(wide) for t in qkv.split([Hq * D, Hkv * D, Hkv * D], dim=1))
+    if cos is not None:
+        if int(pos.max()) >= cos.shape[0]:
+            raise ValueError(f"a document of {int(pos.max()) + 1} tokens, cos / sin for {cos.shape[0]}")
+        c, s = (t[pos.clamp(min=0)].unsqueeze(1).to(wide) for t in (cos, sin))
+        q, k = (torch.cat([a * c - b * s, b * c + a * s], dim=-1) for a, b in (q.chunk(2, -1), k.chunk(2, -1)))
+        q, k = q.to(qkv.dtype).to(wide), k.to(qkv.dtype).to(wide)
+    k, v = k.repeat_interleave(Hq // Hkv, 1), v.repeat_interleave(Hq // Hkv, 1)
+    doc = torch.cumsum(pos == 0, 1)  # a document's tokens follow its first one
+    seen = (doc.unsqueeze(2) == doc.unsqueeze(1)) & (pos >= 0).unsqueeze(2) & (pos >= 0).unsqueeze(1)
+    if causal:
+        seen = seen & (pos.unsqueeze(2) >= pos.unsqueeze(1))
+    inside = (pos >= 0).view(rows, 1, S, 1)
+    # what padding holds (an Inf, say) must not reach a product
+    q, k, v = (torch.where(inside, t, 0.0) for t in (q, k, v))
+    att = (q @ k.transpose(2, 3) * scale).masked_fill(~seen.unsqueeze(1), torch.finfo(wide).min).softmax(-1)
+    out = torch.where(inside, att @ v, 0.0)
+    return out.transpose(1, 2).reshape(rows * S, Hq * D).to(qkv.dtype)
+
+
+# ------------------------------------------------------------------------------------------------
+# dropout
+# ------------------------------------------------------------------------------------------------
+def _philox_numbers(seed: int, stream: int, count: int, device) -> torch.Tensor:
+    """``count`` 16-bit numbers as ``csrc/dropout.cu`` draws them, in 64-bit integer arithmetic."""
+    low = 0xFFFFFFFF
+    block = torch.arange((count + 7) // 8, device=device)
+    x = [block & low, block >> 32, torch.full_like(block, stream & low), torch.full_like(block, (stream >> 32) & low)]
+    k0, k1 = seed & low, (seed >> 32) & low
+    for _ in range(10):
+        a, b = x[0] * 0xD2511F53, x[2] * 0xCD9E8D57  # modulo 2^64: the shift leaves the upper half's bits in place
+        x = [((b >> 32) & low) ^ x[1] ^ k0, b & low, ((a >> 32) & low) ^ x[3] ^ k1, a & low]
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    words = torch.stack(x, 1)
+    return torch.stack([words & 0xFFFF, words >> 16], 2).reshape(-1)[:count]
+
+
+class _DropoutFn(torch.autograd.Function):
+    """The mask is a function of the seed: the backward computes it again.  A seed tensor is a saved tensor, so changing it
+    in place between the two is autograd's usual error."""
+
+    @staticmethod
+    def forward(ctx, x, residual, seed, seed_value: int, stream: int, threshold: int):
+        ctx.save_for_backward(seed)
+        ctx.cfg = (seed_value, stream, threshold)
+        return _DropoutFn.launch(x, residual, seed, seed_value, stream, threshold)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (seed,) = ctx.saved_tensors
+        dx = _DropoutFn.launch(dy, None, seed, *ctx.cfg) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
+
+    @staticmethod
+    def launch(x, residual, seed, seed_value, stream, threshold):
+        x = x.contiguous()
+        residual = None if residual is None else residual.contiguous()
+        y = torch.empty_like(x)
+        with _on_device_of(x):
+            _lib.check(
+                _lib.lib().pb_dropout(_lib.addr(x), _lib.addr(residual), _lib.addr(y), x.numel(), _lib.addr(seed),
+                                      seed_value, stream, threshold, _lib.stream_addr()),
+                "pb_dropout",
+            )
+        return y
+
+
+def dropout(x, p: float, seed: Union[int, torch.Tensor], residual: Optional[torch.Tensor] = None, stream: int = 0):
+    """``x * mask / (1 - p) (+ residual)``, each element dropped with probability ``p`` (rounded to a multiple of 2^-16; the
+    factor uses the rounded value).  The mask is a function of ``(seed, stream, element index)`` by Philox4x32-10 (Salmon et
+    al., SC 2011), the same on every device, and is never stored: the backward computes it again.
+
+    ``seed``: an int, or an int64 tensor of one element on ``x``'s device, read when the kernel runs (a captured graph
+    draws another mask for another seed in it).  ``stream``: a number from 0 to 2^63 - 1 that keeps the layers of one seed
+    apart.  Dropped elements are 0 (or ``residual``) whatever ``x`` holds."""
+    threshold = int(math.floor(p * 65536 + 0.5)) if 0.0 <= p <= 1.0 else -1
+    if not 0 <= threshold <= 65535:
+        raise ValueError(f"p has to be at least 0 and below 1 - 2^-17, got {p}")
+    if not 0 <= stream < 2 ** 63:
+        raise ValueError(f"stream: 0 to 2^63 - 1, got {stream}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"residual: {tuple(x.shape)} {x.dtype} on {x.device}, got {tuple(residual.shape)} "
+                         f"{residual.dtype} on {residual.device}")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+            raise ValueError(f"seed: one int64 on {x.device}, got {tuple(seed.shape)} {seed.dtype} on {seed.device}")
+        seed_value = 0
+    else:
+        seed_value, seed = (int(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63, None  # modulo 2^64, as the kernel's 64 bits hold it
+    if _use_kernels(x):
+        return _DropoutFn.apply(x, residual, seed, seed_value, stream, threshold)
+    number = seed_value if seed is None else int(seed)
+    keep = _philox_numbers(number, stream, x.numel(), x.device).view(x.shape) >= threshold
+    wide = torch.promote_types(x.dtype, torch.float32)
+    y = torch.where(keep, x.to(wide) * (65536.0 / (65536 - threshold)), 0.0)
+    if residual is not None:
+        y = y + residual.to(wide)
+    return y.to(x.dtype)

@@ -1,0 +1,201 @@
+"""Scaled embedding with given positions and its gradient by sorted tokens, against sums in 64 bits."""
+import pytest
+import torch
+
+from pippy_b200.ops import _lib
+from pippy_b200.ops import functional as pf
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -8  # a bf16 rounding is off by at most this much of the value
+F32 = 2.0 ** -24
+
+
+@pytest.fixture
+def errors():
+    yield
+    _lib.check_device_errors()
+
+
+def _sums(keys, rows, size, scale=1.0):
+    """Sums of the rows of each key in 64 bits, sums of their absolute values, and how many there are."""
+    ok = (keys >= 0) & (keys < size)
+    value = torch.zeros(size, rows.shape[1], dtype=torch.float64, device=rows.device)
+    size_of = torch.zeros_like(value)
+    count = torch.zeros(size, 1, dtype=torch.float64, device=rows.device)
+    value.index_add_(0, keys[ok], rows[ok].double() * scale)
+    size_of.index_add_(0, keys[ok], (rows[ok].double() * scale).abs())
+    count.index_add_(0, keys[ok], torch.ones(int(ok.sum()), 1, dtype=torch.float64, device=rows.device))
+    return value, size_of, count
+
+
+def test_plain_form():
+    ids = torch.tensor([[3, 1, 1], [0, 3, 3]])
+    wte, wpe = (torch.randn(n, 8, dtype=torch.float64, requires_grad=True) for n in (4, 3))
+    pos = torch.tensor([0, 1, -1, 2, -1, 0])
+    out = pf.embedding(ids, wte, wpe, 3, scale=2.5, positions=pos)
+    want = 2.5 * wte.detach()[ids.reshape(-1)]
+    want[pos >= 0] += wpe.detach()[pos[pos >= 0]]
+    assert torch.allclose(out, want, rtol=1e-14, atol=0)
+    g = torch.randn_like(out)
+    dw, dp = torch.autograd.grad(out, (wte, wpe), g)
+    assert torch.allclose(dw, _sums(ids.reshape(-1), g, 4, 2.5)[0]) and torch.allclose(dp, _sums(pos, g, 3)[0])
+    assert torch.equal(pf.embedding(ids, wte, wpe, 3, sorted_grad=True), pf.embedding(ids, wte, wpe, 3))
+    assert torch.autograd.gradcheck(lambda a, b: pf.embedding(ids, a, b, 3, scale=2.5, positions=pos), (wte, wpe))
+
+
+def test_refusals():
+    wte = torch.zeros(4, 8)
+    for kw in (dict(positions=torch.zeros(2, dtype=torch.int32)), dict(wpe=wte, positions=torch.zeros(3, dtype=torch.int32)),
+               dict(wpe=wte, positions=torch.zeros(2))):
+        with pytest.raises(ValueError):
+            pf.embedding(torch.tensor([1, 2]), wte, **kw)
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+CASES = {  # tokens, rows of the table, width, share of one id
+    "one": (1, 5, 8, 0.0),
+    "few": (33, 300, 64, 0.0),
+    "one_row": (1000, 1, 72, 0.0),
+    "odd": (3001, 257, 1000, 0.0),
+    "hot": (20_000, 5000, 128, 0.5),
+    "wide": (700, 70_000, 2056, 0.1),
+    "all_one": (5000, 40, 256, 1.0),
+    "long": (200_003, 1 << 17, 16, 0.2),
+}
+
+
+def _ids(T, V, hot, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, V, (T,), generator=gen)
+    ids[torch.rand(T, generator=gen) < hot] = V // 2
+    return ids.cuda(), gen
+
+
+@gpu
+@pytest.mark.parametrize("case", sorted(CASES))
+@pytest.mark.parametrize("buffers", [True, False])
+@pytest.mark.parametrize("given", [True, False])
+def test_kernel(case, buffers, given, errors):
+    T, V, H, hot = CASES[case]
+    S, P, scale = max(1, T // 3), max(1, T // 3) + 2, 1.5
+    ids, gen = _ids(T, V, hot)
+    wte, wpe = (torch.nn.Parameter(torch.randn(n, H, generator=gen).bfloat16().cuda()) for n in (V, P))
+    pos = torch.randint(-1, P, (T,), generator=gen).cuda() if given else torch.arange(T, device="cuda") % S
+    dout = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    start = [torch.randn(p.shape, generator=gen).cuda() for p in (wte, wpe)]
+
+    def call():
+        for p, b in zip((wte, wpe), start):
+            p.grad = None
+            if buffers:
+                p.main_grad = b.clone()
+        out = pf.embedding(ids, wte, wpe, S, scale=scale, positions=pos if given else None, sorted_grad=True)
+        out.backward(dout)
+        return out.detach(), [p.main_grad if buffers else p.grad for p in (wte, wpe)]
+
+    out, grads = call()
+    want = scale * wte.detach().double()[ids]
+    want[pos >= 0] += wpe.detach().double()[pos[pos >= 0]]
+    size = scale * wte.detach().double()[ids].abs() + wpe.detach().double().abs().max()
+    assert ((out.double() - want).abs() <= U * want.abs() + 4 * F32 * size).all()
+    for g, b, keys, factor in zip(grads, start, (ids, pos), (scale, 1.0)):
+        value, magnitude, count = _sums(keys, dout, g.shape[0], factor)
+        # n additions of bf16 values in fp32, a product, one more addition or the rounding to bf16
+        bound = (count + 3) * F32 * magnitude
+        if buffers:
+            value, bound = value + b.double(), bound + 2 * F32 * (value.abs() + b.double().abs())
+            assert g.dtype == torch.float32 and torch.equal(g[count.view(-1) == 0], b[count.view(-1) == 0])
+        else:
+            bound = bound * (1 + U) + U * value.abs()
+            assert g.dtype == torch.bfloat16 and not g[count.view(-1) == 0].any()
+        assert ((g.double() - value).abs() <= bound).all()
+    again = call()
+    assert torch.equal(again[0], out) and all(torch.equal(a, b) for a, b in zip(again[1], grads))
+
+
+@gpu
+def test_kernel_accumulates_and_respects_frozen_tables(errors):
+    ids, gen = _ids(500, 60, 0.1)
+    wte, wpe = (torch.nn.Parameter(torch.randn(n, 32, generator=gen).bfloat16().cuda()) for n in (60, 100))
+    dout = torch.randn(500, 32, generator=gen).bfloat16().cuda()
+    value = _sums(ids, dout, 60)
+    for _ in range(2):  # .grad is added to
+        pf.embedding(ids, wte, seq_len=100, sorted_grad=True).backward(dout)
+    assert ((wte.grad.double() - 2 * value[0]).abs() <= 4 * U * (2 * value[0].abs()) + 200 * F32 * value[1]).all()
+    wte.grad = None
+    wte.requires_grad_(False)
+    pf.embedding(ids, wte, wpe, 100, sorted_grad=True).backward(dout)
+    assert wte.grad is None and wpe.grad is not None
+    pf.embedding(ids, wte, wpe, 100, scale=3.0).backward(dout)
+    wte.requires_grad_(True)
+    wte.main_grad = torch.zeros(60, 32, device="cuda")  # one table with a buffer, one without
+    wpe.grad = None
+    pf.embedding(ids, wte, wpe, 100, sorted_grad=True).backward(dout)
+    assert ((wte.main_grad.double() - value[0]).abs() <= U * value[0].abs() + 500 * F32 * value[1]).all()
+    assert wpe.grad is not None
+    with torch.no_grad():
+        assert pf.embedding(ids[:0], wte, wpe, 100, sorted_grad=True).shape == (0, 32)
+
+
+@gpu
+def test_kernel_reports_bad_ids():
+    ids = torch.tensor([3, -1, 60, 5, 2 ** 40], device="cuda")
+    wte = torch.nn.Parameter(torch.ones(60, 16, device="cuda").bfloat16())
+    out = pf.embedding(ids, wte, scale=2.0)
+    out.backward(torch.ones_like(out))
+    assert torch.equal(out[:, 0].float().cpu(), torch.tensor([2.0, 0, 0, 2.0, 0]))
+    assert wte.grad.sum() == 2 * 16 * 2.0
+    with pytest.raises(_lib.KernelError, match="code 5"):
+        _lib.check_device_errors()
+    wpe = torch.ones(4, 16, device="cuda").bfloat16()
+    out = pf.embedding(ids[:1].repeat(3), wte, wpe, positions=torch.tensor([-1, 3, 4], device="cuda"))
+    assert torch.equal(out[:, 0].float().cpu(), torch.tensor([1.0, 2.0, 1.0]))
+    with pytest.raises(_lib.KernelError, match="code 5"):
+        _lib.check_device_errors()
+    with pytest.raises(ValueError):
+        pf.embedding(ids.cpu(), wte, scale=2.0)
+    with pytest.raises(ValueError):
+        pf.embedding(ids, torch.ones(60, 12, device="cuda").bfloat16(), scale=2.0)
+
+
+@gpu
+def test_kernel_streams_graph_and_deferral(errors):
+    from pippy_b200.backward import DeferredWeightGrads, defer_weight_grads
+
+    T, V, H = 4000, 900, 256
+    cases = []
+    for seed in (1, 2):
+        ids, gen = _ids(T, V, 0.2, seed)
+        cases.append((ids, torch.randn(T, H, generator=gen).bfloat16().cuda()))
+    wte = torch.nn.Parameter(torch.randn(V, H).bfloat16().cuda())
+
+    def call(ids, dout):
+        table = torch.nn.Parameter(wte.detach())
+        table.main_grad = torch.zeros(V, H, device="cuda")
+        pf.embedding(ids, table, sorted_grad=True).backward(dout)
+        return table.main_grad
+
+    want = [call(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], []
+    for _ in range(3):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, call(*c)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i, g in got)
+    ids, dout = cases[0][0].clone(), cases[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(ids, dout)
+    for i in (1, 0):
+        ids.copy_(cases[i][0]), dout.copy_(cases[i][1])
+        graph.replay()
+        assert torch.equal(out, want[i])
+    wte.main_grad = torch.zeros(V, H, device="cuda")
+    queue = DeferredWeightGrads()
+    with defer_weight_grads(queue):
+        pf.embedding(cases[0][0], wte, sorted_grad=True).backward(cases[0][1])
+    assert not wte.main_grad.any()
+    queue.run()
+    assert torch.equal(wte.main_grad, want[0])
