@@ -8,6 +8,8 @@
 #include <string.h>
 
 extern "C" void pb_count_launch(int n);
+extern "C" int pb_device_sm_count();
+extern "C" int pb_get_sm_reserve();
 
 namespace pbv {
 
@@ -29,47 +31,114 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&w);
 }
 
+template <bool V>
+struct Flag {
+  static constexpr bool value = V;
+};
+
 // A warp's wait: every lane waits, all take the same branch.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
-// Loads a tile of 128 rows (kChunks chunks of 64 columns) for the whole warp.  A tile that reaches beyond its document
-// (`valid` < 128 rows) also brings rows of the next one, and an Inf or NaN there would spread: 0 * NaN is NaN in the products
-// that contract over these rows.  Such a tile is waited for here (on `aux`, whose phase the caller tracks), its foreign rows
-// are cleared, and only then is `full` completed.  Happens once per document and operand.
+// ------------------------------------------------------------------------------------------------ pairs of fp32 values
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of a pair on the FMA pipe, where the special-function unit (16 results a clock and SM) is what bounds a softmax.
+// x = n + f with n the nearest integer, read from the low bits of x + 1.5 * 2^23; 2^f on [-1/2, 1/2] by the polynomial of
+// degree 4 whose largest relative error is least (2.7e-6 in fp32; the exchange algorithm of Remez); times 2^n by its
+// exponent bits.  x below -126 gives 2^-126 and not 0; NaN stays NaN.
+__device__ __forceinline__ f32x2 poly_exp2(f32x2 x) {
+  float2 v = both(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
+  x = pair(v.x, v.y);
+  const f32x2 t = add2(x, pair(12582912.f, 12582912.f));
+  const f32x2 n = add2(t, pair(-12582912.f, -12582912.f));
+  const f32x2 f = fma2(n, pair(-1.f, -1.f), x);
+  f32x2 p = pair(9.570102e-3f, 9.570102e-3f);
+  p = fma2(p, f, pair(5.591786e-2f, 5.591786e-2f));
+  p = fma2(p, f, pair(0.24024744f, 0.24024744f));
+  p = fma2(p, f, pair(0.6931218f, 0.6931218f));
+  p = fma2(p, f, pair(0.9999993f, 0.9999993f));
+  const float2 b = both(t);
+  const f32x2 e = pair(__uint_as_float((__float_as_uint(b.x) << 23) + 0x3f800000u),
+                       __uint_as_float((__float_as_uint(b.y) << 23) + 0x3f800000u));
+  return mul2(p, e);
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+// Issues the load of a tile of 128 rows (kChunks chunks of 64 columns); one thread.
 template <int kChunks>
-__device__ __forceinline__ bool load_tile(uint8_t* dst, const CUtensorMap* tm, uint64_t* full, uint64_t* aux,
-                                          uint32_t* aux_phase, int col, int row, int valid, int lane,
-                                          volatile int* abort_flag) {
-  const bool whole = valid >= 128;
-  uint64_t* bar = whole ? full : aux;
-  if (lane == 0) {
-    mbar_expect_tx(bar, kChunks * kChunkBytes);
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, uint64_t* bar, int col, int row) {
+  mbar_expect_tx(bar, kChunks * kChunkBytes);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) tma_load_2d(dst + c * kChunkBytes, tm, bar, col + c * 64, row);
-  }
-  __syncwarp();
-  if (whole) return true;
-  const bool ok = warp_wait(aux, *aux_phase, abort_flag);
-  *aux_phase ^= 1;
-  if (!ok) return false;
-  // a row is 128 contiguous bytes of each chunk; the swizzle only permutes inside it
+  for (int c = 0; c < kChunks; ++c) tma_load_2d(dst + c * kChunkBytes, tm, bar, col + c * 64, row);
+}
+
+// A tile that reaches beyond its document (`valid` < 128 rows) also brings rows of the next one, and an Inf or NaN there would
+// spread: 0 * NaN is NaN in the products that contract over these rows.  So it is loaded against a barrier of its own
+// (`raw`), on which a warp waits that clears the foreign rows and only then completes `full`.  A row is 128
+// contiguous bytes of each chunk; the swizzle only permutes inside it.
+template <int kChunks>
+__device__ __forceinline__ void clear_tail(uint8_t* tile, int valid, uint64_t* full, int lane) {
 #pragma unroll
   for (int c = 0; c < kChunks; ++c)
     for (int at = valid * 128 + lane * 16; at < kChunkBytes; at += 512)
-      *reinterpret_cast<uint4*>(dst + c * kChunkBytes + at) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(tile + c * kChunkBytes + at) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) mbar_arrive(full);
-  return true;
 }
 
-// Zeros in rows [first, stop) x D columns of a padding tile; all threads of the block.
+// The blocks of a launch stay and take the work items i = 0, 1, ... (tile of the table, head; longest first) in turns, every
+// other turn in reverse, so that no block gets the longer item of every turn.  All roles of a block walk the same sequence.
+struct Items {
+  int n, turn, i;
+  __device__ __forceinline__ explicit Items(int count) : n(count), turn(-1), i(0) {}
+  // next item of this block, -1 after the last
+  __device__ __forceinline__ int next() {
+    for (;;) {
+      ++turn;
+      const long long first = (long long)turn * gridDim.x;
+      if (first >= n) return -1;
+      i = (int)first + ((turn & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+      if (i < n) return i;
+    }
+  }
+};
+
+// Zeros in `rows` rows x D columns of a padding tile, by `threads` threads.
 template <int D>
-__device__ __forceinline__ void clear_rows(__nv_bfloat16* base, long long stride, long long first, int rows, int col) {
+__device__ __forceinline__ void clear_rows(__nv_bfloat16* base, long long stride, long long first, int rows, int col,
+                                           int thread, int threads) {
   constexpr int kVec = D / 8;
-  for (int i = threadIdx.x; i < rows * kVec; i += blockDim.x)
+  for (int i = thread; i < rows * kVec; i += threads)
     *reinterpret_cast<uint4*>(base + (first + i / kVec) * stride + col + (i % kVec) * 8) = make_uint4(0, 0, 0, 0);
 }
 
@@ -83,6 +152,13 @@ __device__ __forceinline__ void leave(volatile int* abort_flag, int warp, uint32
   tc_fence_after_sync();
   __syncwarp();
   if (warp == 1) tmem_dealloc<1>(tmem_base, 512);
+}
+
+// Blocks of a launch that stays resident: one per SM that is not reserved for others, no more than there are items.
+inline unsigned resident_blocks(long long items) {
+  int sms = pb_device_sm_count() - pb_get_sm_reserve();
+  if (sms < 1) sms = 1;
+  return (unsigned)(items < sms ? items : sms);
 }
 
 }  // namespace pbv

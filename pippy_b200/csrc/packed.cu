@@ -11,8 +11,10 @@ namespace pbk {
 
 // Tiles are listed longest first: tile `rank` of a document sees rank + 1 tiles of keys (as a tile of keys it is seen by as
 // many tiles of queries when counted from the document's end), and a long tile that starts last runs alone at the end.
-// Ranks above the last bucket share it; they are all long.
-constexpr int kBuckets = 2048;
+// Ranks above the last bucket share it; they are all long.  Behind rank 0 come, in the table of 256 rows, the documents that
+// fill no more than half a tile (the attention forward takes two heads of such a one at a time), and then the padding.
+constexpr int kRanks = 2048;
+constexpr int kBuckets = kRanks + 1;  // the last one; padding's is kBuckets
 constexpr int kPlanThreads = 1024;
 constexpr int kChunk = 4096;  // tokens a block writes positions for
 
@@ -23,7 +25,7 @@ struct LayoutArgs {
   int2* segments;  // [rows * (docs + 1)]: start, length; the last of a row is its padding
   Tile* tiles[2];  // of 128 and of 256 rows
   int max_tiles[2];
-  int* counts;  // [2]
+  int* counts;  // [table][all, those before the half-filled ones, those before the padding]
   int* err;
 };
 
@@ -74,7 +76,8 @@ __device__ void plan_tiles(const LayoutArgs& a, int* s_hist, int* s_part) {
         const bool pad = i % (a.docs + 1) == a.docs;
         const int n = (seg.y + tile_rows - 1) / tile_rows;
         for (int r = lane; r < n; r += 32) {
-          const int bucket = pad ? kBuckets : kBuckets - 1 - min(r, kBuckets - 1);  // high ranks first
+          const bool half = table == 1 && seg.y <= 128;
+          const int bucket = pad ? kBuckets : (half ? kRanks : kRanks - 1 - min(r, kRanks - 1));  // high ranks first
           const int at = atomicAdd(&s_hist[bucket], 1);
           if (sweep == 1 && at < a.max_tiles[table]) a.tiles[table][at] = Tile{seg.x, seg.y, r, pad ? 1 : 0};
         }
@@ -103,7 +106,12 @@ __device__ void plan_tiles(const LayoutArgs& a, int* s_hist, int* s_part) {
             base += n;
           }
         }
-        if (tid == kPlanThreads - 1) a.counts[table] = min(base, a.max_tiles[table]);
+        if (tid == kPlanThreads - 1) a.counts[table * 4] = min(base, a.max_tiles[table]);
+        __syncthreads();
+        if (tid == 0) {
+          a.counts[table * 4 + 1] = min(s_hist[kRanks], a.max_tiles[table]);
+          a.counts[table * 4 + 2] = min(s_hist[kBuckets], a.max_tiles[table]);
+        }
         __syncthreads();
       }
     }
@@ -190,7 +198,7 @@ __global__ void __launch_bounds__(256) packed_rope_kernel(const __nv_bfloat16* s
 extern "C" {
 
 // lengths [rows, docs] -> positions [rows * seq] (-1 in padding), segments [rows * (docs + 1)] pairs, tile tables of 128 and
-// 256 rows (max128 / max256 entries of 4 ints; the host takes an upper bound), counts [2].
+// 256 rows (max128 / max256 entries of 4 ints; the host takes an upper bound), counts [2][4].
 int pb_packed_layout(const int* lengths, int rows, int docs, int seq, int* positions, int* segments, int* tiles128,
                      int max128, int* tiles256, int max256, int* counts, int* err_dev, void* stream_) {
   using namespace pbk;

@@ -735,12 +735,12 @@ def packed_layout(lengths: torch.Tensor, tokens_per_row: int) -> PackedLayout:
         segments = rows * (docs + 1)
         most = {n: rows * S // n + min(segments, rows * S) for n in (128, 256)}
         # one buffer, every part on a 16-byte boundary: tiles of 4 ints, then segments, counts, positions
-        ints = 4 * (most[128] + most[256]), (2 * segments + 3) // 4 * 4, 4
+        ints = 4 * (most[128] + most[256]), (2 * segments + 3) // 4 * 4, 8
         buf = torch.empty(sum(ints) + rows * S, dtype=torch.int32, device=lengths.device)
         tiles, segs, counts, positions = buf.split([*ints, rows * S])
         layout = PackedLayout(given, S, positions)
         layout.tiles = {128: tiles[: 4 * most[128]], 256: tiles[4 * most[128]:]}
-        layout.max_tiles, layout.counts = most, {128: counts[:1], 256: counts[1:2]}
+        layout.max_tiles, layout.counts = most, {128: counts[:4], 256: counts[4:]}
         _lib.check(
             _lib.lib().pb_packed_layout(_lib.addr(given), rows, docs, S, _lib.addr(positions), _lib.addr(segs),
                                         _lib.addr(layout.tiles[128]), most[128], _lib.addr(layout.tiles[256]), most[256],

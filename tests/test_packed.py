@@ -155,7 +155,7 @@ def test_refusals():
 
 # ------------------------------------------------------------------------------------------------ GPU
 def _read_tiles(layout, rows):
-    n = int(layout.counts[rows])
+    n = int(layout.counts[rows][0])
     return layout.tiles[rows][: 4 * n].view(n, 4).tolist()
 
 
@@ -184,6 +184,9 @@ def test_layout_kernel(case, errors):
         assert len(got) == len(want) <= layout.max_tiles[rows] and {tuple(t) for t in got} == want
         ranks = [t[2] if not t[3] else -1 for t in got]  # longest first, as far as there are buckets; padding last
         assert all(a >= b or min(a, b) >= 2047 for a, b in zip(ranks, ranks[1:]) if b >= 0) and sorted(ranks, key=lambda t: t == -1) == ranks
+        half = [rows == 256 and t[1] <= 128 and not t[3] for t in got]  # the last ones before the padding
+        n_first, n_docs = layout.counts[rows][1:3].tolist()
+        assert n_docs == sum(1 for t in got if not t[3]) and half == [n_first <= i < n_docs for i in range(len(got))]
 
 
 @gpu
@@ -226,6 +229,26 @@ def test_attention_kernel(lengths, S, heads, D, causal, rotary, errors):
         assert torch.isfinite(a).all() and ((a.double() - b).abs() <= bound).all()
     again = _run(qkv, do, cos, sin, layout, hq, hk, D, causal=causal)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(16, 16), (12, 4), (15, 5)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_kernel_many_items(heads, D, errors):
+    """Every resident block walks a dozen work items: documents of one block, of two and three, padding between them."""
+    gen = torch.Generator().manual_seed(7)
+    lengths = [torch.randint(0, 120, (30,), generator=gen).tolist() for _ in range(4)]
+    lengths[1][3:6], lengths[2][0] = [128, 129, 400], 256
+    S = max(sum(row) for row in lengths) + 17
+    hq, hk = heads
+    qkv, do, cos, sin = _inputs(lengths, S, hq, hk, D, True, "cuda")
+    layout = _layout(lengths, S, "cuda")
+    got = _run(qkv, do, cos, sin, layout, hq, hk, D)
+    want = _definition(qkv, do, lengths, S, hq, hk, D, cos, sin)
+    for a, (b, bound) in zip(got, want):
+        assert torch.isfinite(a).all() and ((a.double() - b).abs() <= bound).all()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(got, _run(qkv, do, cos, sin, layout, hq, hk, D)))
 
 
 @gpu
