@@ -36,6 +36,17 @@ struct Flag {
   static constexpr bool value = V;
 };
 
+// Moves registers between the warpgroups of a block: all four warps of a warpgroup call it, and over the block the shares add
+// up to no more than what it was launched with (threads x registers each), or the increase would wait for good.
+template <int N>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // A warp's wait: every lane waits, all take the same branch.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
@@ -153,6 +164,33 @@ __device__ __forceinline__ void leave(volatile int* abort_flag, int warp, uint32
   __syncwarp();
   if (warp == 1) tmem_dealloc<1>(tmem_base, 512);
 }
+
+// Items of a table of tiles and heads (tile_order), with the next one's table entry on its way while one is worked on: the
+// read of the table took 1 000 cycles between two items.
+struct Walk {
+  Items items;
+  const Tile* tiles;
+  int count, heads, group;
+  int i, head;
+  Tile tile;
+  __device__ __forceinline__ Walk(const Tile* tiles, int count, int heads, int group)
+      : items(count * heads), tiles(tiles), count(count), heads(heads), group(group) {
+    fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    if ((i = items.next()) < 0) return;
+    const TileOrder order = tile_order(i, count, heads, group);
+    head = order.index;
+    tile = tiles[order.tile_rank];
+  }
+  __device__ __forceinline__ bool next(Tile& t, int& h) {
+    if (i < 0) return false;
+    t = tile;
+    h = head;
+    fetch();
+    return true;
+  }
+};
 
 // Blocks of a launch that stays resident: one per SM that is not reserved for others, no more than there are items.
 inline unsigned resident_blocks(long long items) {

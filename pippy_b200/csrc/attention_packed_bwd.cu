@@ -48,7 +48,7 @@ struct BwdArgs {
 };
 
 // kPolyPairs of 8 pairs of exponentials are computed on the FMA pipe (poly_exp2)
-constexpr int kPolyPairs = 3;
+constexpr int kPolyPairs = 4;
 
 __device__ __forceinline__ f32x2 exp2_pair(f32x2 x, bool poly) {
   if (poly) return poly_exp2(x);
@@ -56,51 +56,97 @@ __device__ __forceinline__ f32x2 exp2_pair(f32x2 x, bool poly) {
   return pair(fast_exp2(v.x), fast_exp2(v.y));
 }
 
-// One row of an accumulator [128, D] to bf16: this warp's columns are [sub * D / 4, + D / 4) of each half, so that a thread
-// holds both elements of every pair that the rotation mixes.  `pos` < 0: no rotation to undo.
+// Mask of a packed pair of bf16 of which the first `n` values stay (all for n >= 2, none for n <= 0).
+__device__ __forceinline__ uint32_t keep_below(int n) {
+  uint32_t m;
+  asm("shr.u32 %0, 0xffffffff, %1;" : "=r"(m) : "r"(max(32 - 16 * n, 0)));  // shifts by 32 and more give 0
+  return m;
+}
+
+// A warp's share of the rotation tables for 32 rows: columns [sub * D / 4, + D / 4) of each, on its way from memory while the
+// products that it is for are still running.  pos: position of the first row, < 0 for no rotation; rows: how many of the 32 are
+// the document's.
 template <int D>
-__device__ __forceinline__ void write_row(uint32_t acc, int sub, float scale, const BwdArgs& p, int pos, bool row_ok,
-                                          __nv_bfloat16* dst) {
-  constexpr int N = D / 4;
-  const bool turn = pos >= 0 && pos < p.table_rows;
-  const long long at = turn ? (long long)pos * (D / 2) + sub * N : 0;
+struct Turn {
+  static constexpr int kChunks = D / 64;  // of 16 columns
+  float4 cs[kChunks][4], sn[kChunks][4];
+  __device__ __forceinline__ void fetch(const BwdArgs& p, int pos, int rows, int sub, int lane) {
 #pragma unroll
-  for (int c0 = 0; c0 < N; c0 += 16) {
-    uint32_t a[16], b[16];
-    tmem_ld_32x16(acc + sub * N + c0, a);
-    tmem_ld_32x16(acc + D / 2 + sub * N + c0, b);
-    float4 cs[4], sn[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      cs[u] = turn ? __ldg(reinterpret_cast<const float4*>(p.cs + at + c0) + u) : make_float4(1.f, 1.f, 1.f, 1.f);
-      sn[u] = turn ? __ldg(reinterpret_cast<const float4*>(p.sn + at + c0) + u) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    tmem_ld_wait();
-    if (row_ok) {
-      uint32_t lo[8], hi[8];
+    for (int c = 0; c < kChunks; ++c)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float c[4] = {cs[u].x, cs[u].y, cs[u].z, cs[u].w}, n[4] = {sn[u].x, sn[u].y, sn[u].z, sn[u].w};
-        float x[4], y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float f = __uint_as_float(a[u * 4 + i]) * scale, g = __uint_as_float(b[u * 4 + i]) * scale;
-          x[i] = f * c[i] + g * n[i];
-          y[i] = g * c[i] - f * n[i];
-        }
-        lo[u * 2] = pack_bf16(x[0], x[1]), lo[u * 2 + 1] = pack_bf16(x[2], x[3]);
-        hi[u * 2] = pack_bf16(y[0], y[1]), hi[u * 2 + 1] = pack_bf16(y[2], y[3]);
+        const int r = u * 8 + (lane >> 2);
+        const bool in = pos >= 0 && r < rows && pos + r < p.table_rows;
+        const long long at = (long long)(pos + r) * (D / 2) + sub * (D / 4) + c * 16 + (lane & 3) * 4;
+        cs[c][u] = in ? __ldg(reinterpret_cast<const float4*>(p.cs + at)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        sn[c][u] = in ? __ldg(reinterpret_cast<const float4*>(p.sn + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      __nv_bfloat16* at_lo = dst + sub * N + c0;
-      __nv_bfloat16* at_hi = at_lo + D / 2;
+  }
+};
+
+// 32 rows of an accumulator [128, D] to bf16, by one warp, a row per lane.  The warp's columns are [sub * D / 4, + D / 4) of each
+// half, so that a thread holds both elements of every pair that the rotation mixes.  A lane that read and wrote its
+// own row in global memory touched 32 lines with every access: 6 000 to 9 000 cycles for a tile of 128 x 128, several times
+// what its products take.  So the tables come, and the results leave, through `stage` (32 * D bytes of the warp's own), as
+// segments of 64 bytes.
+template <int D, bool kTurn>
+__device__ __forceinline__ void write_rows(uint32_t acc, int sub, float scale, const Turn<D>& turn, int rows, uint8_t* stage,
+                                           int lane, __nv_bfloat16* dst, long long stride) {
+  constexpr int N = D / 4;
+  constexpr int kPieces = D / 16;  // 16-byte pieces of a row's results
+  uint32_t out[N];                 // [half][N / 2]
+  // 64-byte rows: two of them share 128 bytes, hence the shift
+  auto at64 = [&](int row, int piece) { return reinterpret_cast<float4*>(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)); };
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        reinterpret_cast<uint4*>(at_lo)[u] = make_uint4(lo[u * 4], lo[u * 4 + 1], lo[u * 4 + 2], lo[u * 4 + 3]);
-        reinterpret_cast<uint4*>(at_hi)[u] = make_uint4(hi[u * 4], hi[u * 4 + 1], hi[u * 4 + 2], hi[u * 4 + 3]);
+  for (int c = 0; c < N / 16; ++c) {
+    uint32_t a[16], b[16];
+    tmem_ld_32x16(acc + sub * N + c * 16, a);
+    tmem_ld_32x16(acc + D / 2 + sub * N + c * 16, b);
+    float4 cs[4], sn[4];
+    if (kTurn) {
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) *at64(u * 8 + (lane >> 2), lane & 3) = which == 0 ? turn.cs[c][u] : turn.sn[c][u];
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) (which == 0 ? cs[u] : sn[u]) = *at64(lane, u);
+        __syncwarp();
       }
     }
-    __syncwarp();  // the next load of TMEM is one of the whole warp
+    tmem_ld_wait();
+    const f32x2 scale2 = pair(scale, scale);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      f32x2 f = mul2(pair(__uint_as_float(a[u * 2]), __uint_as_float(a[u * 2 + 1])), scale2);
+      f32x2 g = mul2(pair(__uint_as_float(b[u * 2]), __uint_as_float(b[u * 2 + 1])), scale2);
+      if (kTurn) {
+        const f32x2 cc = (u & 1) ? pair(cs[u >> 1].z, cs[u >> 1].w) : pair(cs[u >> 1].x, cs[u >> 1].y);
+        const f32x2 ss = (u & 1) ? pair(sn[u >> 1].z, sn[u >> 1].w) : pair(sn[u >> 1].x, sn[u >> 1].y);
+        const f32x2 x = fma2(g, ss, mul2(f, cc));
+        g = fma2(mul2(f, pair(-1.f, -1.f)), ss, mul2(g, cc));
+        f = x;
+      }
+      const float2 x = both(f), y = both(g);
+      out[c * 8 + u] = pack_bf16(x.x, x.y);
+      out[N / 2 + c * 8 + u] = pack_bf16(y.x, y.y);
+    }
   }
+  auto at = [&](int row, int piece) {
+    const int x = kPieces == 8 ? (row & 7) : ((row >> 1) & 3);
+    return reinterpret_cast<uint4*>(stage + row * (kPieces * 16) + ((piece ^ x) << 4));
+  };
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) *at(lane, u) = make_uint4(out[u * 4], out[u * 4 + 1], out[u * 4 + 2], out[u * 4 + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int r = i * (32 / kPieces) + lane / kPieces, u = lane % kPieces;
+    const uint4 w = *at(r, u);
+    const int col = (u < kPieces / 2 ? 0 : D / 2) + sub * N + (u % (kPieces / 2)) * 8;
+    if (r < rows) *reinterpret_cast<uint4*>(dst + r * stride + col) = w;
+  }
+  __syncwarp();
 }
 
 // ------------------------------------------------------------------------------------------------ pass 1: dQ
@@ -127,7 +173,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint8_t* sK = sDO + TILE_BYTES;
   uint8_t* sV = sK + kStagesK * TILE_BYTES;
   float* s_stat = reinterpret_cast<float*>(sV + kStagesV * TILE_BYTES);  // [item & 1][lse2, delta][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_stat + 512);
+  float* s_delta = s_stat + 512;                                         // [128] delta of the item that is being brought
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_delta + 128);
   uint64_t* stage_full = bars;       // Q and dO of an item are in shared memory
   uint64_t* stage_empty = bars + 1;  // ... and have been taken to TMEM
   uint64_t* res_ready = bars + 2;    // Q, dO in TMEM; lse and delta in s_stat
@@ -165,7 +212,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     for (int i = 0; i < kStagesV; ++i) {
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 8);
     }
     mbar_init(s_full, 1);
     mbar_init(s_read, 8);
@@ -187,16 +234,19 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t tAcc = tmem_base + 384;  // D columns
 
   bool ok = true;
-  Items items(count * p.Hq);
+  Walk walk(p.tiles, count, p.Hq, p.head_group);
+  Tile tile;
+  int h;
   int it = 0;  // items with work so far
   int n = 0;   // blocks so far
-  if (warp == 0) {
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
-      const Tile tile = p.tiles[order.tile_rank];
+  // launched with 128 registers a thread: 64 + 2 x 168 + 112 = 4 x 128
+  if (warp < 4) {
+    give_registers<64>();
+    if (warp == 0) {
+    while (ok && walk.next(tile, h)) {
       const int nblk = blocks_of(tile);
       if (nblk == 0) continue;
-      const int h = order.index, hkv = h / G;
+      const int hkv = h / G;
       if (!(ok = warp_wait(stage_empty, (it & 1) ^ 1, abort_flag))) break;
       if (lane == 0) {
         mbar_expect_tx(stage_full, 2 * TILE_BYTES);
@@ -228,32 +278,30 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       return got;
     };
     // scores: A = resident bf16 rows in TMEM, B = streamed tile, K-major
-    auto issue_scores = [&](uint32_t dst, uint32_t a, const uint8_t* tile_b, uint64_t* full, uint64_t* empty, uint64_t* last) {
+    auto issue_scores = [&](uint32_t dst, uint32_t a, const uint8_t* tile_b, uint64_t* full, uint64_t* last) {
       const uint64_t bd = make_smem_desc(smem_u32(tile_b), 16, 1024);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           umma_ts(dst, a + kk * 8, bd + (((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4), idesc_t, kk != 0);
         umma_commit(full);
-        if (empty) umma_commit(empty);
         if (last) umma_commit(last);
       }
       __syncwarp();
     };
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
-      const int nblk = blocks_of(p.tiles[order.tile_rank]);
+    while (ok && walk.next(tile, h)) {
+      const int nblk = blocks_of(tile);
       if (nblk == 0) continue;
       if (!(ok = wait(res_ready, it & 1) && wait(&k_full[n % kStagesK], (n / kStagesK) & 1))) break;
-      issue_scores(tS, tQ, sK + (n % kStagesK) * TILE_BYTES, s_full, nullptr, nullptr);
+      issue_scores(tS, tQ, sK + (n % kStagesK) * TILE_BYTES, s_full, nullptr);
       if (!(ok = wait(&v_full[n % kStagesV], (n / kStagesV) & 1))) break;
-      issue_scores(tDP, tDO, sV + (n % kStagesV) * TILE_BYTES, dp_full, &v_empty[n % kStagesV], nblk == 1 ? res_empty : nullptr);
+      issue_scores(tDP, tDO, sV + (n % kStagesV) * TILE_BYTES, dp_full, nblk == 1 ? res_empty : nullptr);
       for (int j = 0; j < nblk; ++j, ++n) {
         const bool more = j + 1 < nblk;
         const int m = n + 1;
         if (more) {
           if (!(ok = wait(&k_full[m % kStagesK], (m / kStagesK) & 1) && wait(s_read, n & 1))) break;
-          issue_scores(tS, tQ, sK + (m % kStagesK) * TILE_BYTES, s_full, nullptr, nullptr);
+          issue_scores(tS, tQ, sK + (m % kStagesK) * TILE_BYTES, s_full, nullptr);
           // what the next scores need is waited for while there is nothing to issue anyway
           if (!(ok = wait(&v_full[m % kStagesV], (m / kStagesV) & 1))) break;
         }
@@ -268,15 +316,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         __syncwarp();
         if (more)
-          issue_scores(tDP, tDO, sV + (m % kStagesV) * TILE_BYTES, dp_full, &v_empty[m % kStagesV],
-                       j + 2 == nblk ? res_empty : nullptr);
+          issue_scores(tDP, tDO, sV + (m % kStagesV) * TILE_BYTES, dp_full, j + 2 == nblk ? res_empty : nullptr);
       }
       ++it;
     }
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the k_raw barriers
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Tile tile = p.tiles[tile_order(i, count, p.Hq, p.head_group).tile_rank];
+    while (ok && walk.next(tile, h)) {
       const int nblk = blocks_of(tile);
       if (nblk == 0) continue;
       n += nblk;
@@ -287,42 +333,59 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       phases ^= 1u << sk;
       clear_tail<NCH>(sK + sk * TILE_BYTES, valid, &k_full[sk], lane);
     }
+    }
   } else if (warp >= 12) {
+    give_registers<112>();
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
-      const Tile tile = p.tiles[order.tile_rank];
+    while (ok && walk.next(tile, h)) {
       if (blocks_of(tile) == 0) continue;
-      const int h = order.index;
       const bool row_ok = tile.rank * 128 + r < tile.len;
       const long long row = (long long)tile.start + tile.rank * 128 + r;
       const float lse2 = row_ok ? p.lse[(long long)h * p.T + row] * kLog2e : 0.f;
-      const uint4* o_row = reinterpret_cast<const uint4*>(p.o + row * p.o_stride + h * D);
+      // delta = dO O: D / 8 lanes to a row, so that O is read in whole lines, all of them on their way before dO is waited for
+      constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+      const int u = lane % kLanes, first = quarter * 32 + lane / kLanes;
+      uint4 y[kLanes];
+#pragma unroll
+      for (int k = 0; k < kLanes; ++k)
+        y[k] = tile.rank * 128 + first + k * kRows < tile.len
+                   ? __ldg(reinterpret_cast<const uint4*>(p.o + ((long long)tile.start + tile.rank * 128 + first + k * kRows) * p.o_stride + h * D) + u)
+                   : make_uint4(0, 0, 0, 0);
       if (!(ok = warp_wait(stage_full, it & 1, abort_flag))) break;
       // 16-byte piece u of a row's 128 bytes lies at u ^ (row & 7)
-      auto piece = [&](const uint8_t* tile_s, int u) {
-        return *reinterpret_cast<const uint4*>(tile_s + (u >> 3) * kChunkBytes + r * 128 + (((u & 7) ^ (r & 7)) << 4));
+      auto piece = [&](const uint8_t* tile_s, int row_t, int u) {
+        return *reinterpret_cast<const uint4*>(tile_s + (u >> 3) * kChunkBytes + row_t * 128 + (((u & 7) ^ (row_t & 7)) << 4));
       };
-      float delta = 0.f;
+      float dot[kLanes];
 #pragma unroll
-      for (int u0 = 0; u0 < D / 8; u0 += 8) {
-        uint4 y[8];
+      for (int k = 0; k < kLanes; ++k) {
+        const uint4 x = piece(sDO, first + k * kRows, u);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+        f32x2 sum = pair(0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) y[u] = row_ok ? __ldg(o_row + u0 + u) : make_uint4(0, 0, 0, 0);
+        for (int e = 0; e < 4; ++e)  // a bf16 is the upper half of its fp32
+          sum = fma2(pair(__uint_as_float(xs[e] << 16), __uint_as_float(xs[e] & 0xffff0000u)),
+                     pair(__uint_as_float(ys[e] << 16), __uint_as_float(ys[e] & 0xffff0000u)), sum);
+        const float2 v = both(sum);
+        dot[k] = v.x + v.y;
+      }
+      // the kLanes sums of every lane, added over the lanes of a row: each step halves the sums that a lane still carries, and
+      // lane u ends with row u of its half warp's
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const uint4 x = piece(sDO, u0 + u);
-          const __nv_bfloat162* xb = reinterpret_cast<const __nv_bfloat162*>(&x);
-          const __nv_bfloat162* yb = reinterpret_cast<const __nv_bfloat162*>(&y[u]);
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        const bool upper = u & o;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = __bfloat1622float2(xb[e]), g = __bfloat1622float2(yb[e]);
-            delta += f.x * g.x + f.y * g.y;
-          }
+        for (int k = 0; k < o; ++k) {
+          const float keep = upper ? dot[k + o] : dot[k], give = upper ? dot[k] : dot[k + o];
+          dot[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
         }
       }
+      s_delta[first + u * kRows] = dot[0];
+      __syncwarp();
+      const float delta = s_delta[r];
+      __syncwarp();
       if (row_ok) p.delta[(long long)h * p.T + row] = delta;
       if (!(ok = warp_wait(res_empty, (it & 1) ^ 1, abort_flag))) break;
       tc_fence_after_sync();
@@ -336,7 +399,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           uint32_t w[32];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const uint4 x = piece(which == 0 ? sQ : sDO, c * 8 + u);
+            const uint4 x = piece(which == 0 ? sQ : sDO, r, c * 8 + u);
             w[u * 4] = x.x, w[u * 4 + 1] = x.y, w[u * 4 + 2] = x.z, w[u * 4 + 3] = x.w;
           }
           tmem_st_32x32((which == 0 ? tQ : tDO) + lane_off + c * 32, w);
@@ -350,17 +413,16 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       ++it;
     }
-  } else if (warp >= 4) {
+  } else {
+    take_registers<168>();
     const int sub = (warp - 4) >> 2;  // 0, 1: columns [64 sub, 64 sub + 64) of a block
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t my_s = tS + lane_off + sub * 64, my_dp = tDP + lane_off + sub * 64;
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
-      const Tile tile = p.tiles[order.tile_rank];
+    while (ok && walk.next(tile, h)) {
       const int nblk = blocks_of(tile);
-      const int h = order.index, q0 = tile.rank * 128, q_idx = q0 + r;
+      const int q0 = tile.rank * 128, q_idx = q0 + r;
       if (nblk == 0) {
         clear_rows<D>(p.out_a, p.out_stride, (long long)tile.start + q0, min(128, tile.len - q0), h * D, threadIdx.x - 128, 256);
         continue;
@@ -373,49 +435,42 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       for (int j = 0; j < nblk; ++j, ++n) {
         if (!(ok = warp_wait(s_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
+        uint32_t t[2][32];
         f32x2 pr[32];
-        {
-          uint32_t t[2][32];
-          tmem_ld_32x32(my_s, t[0]);
-          tmem_ld_32x32(my_s + 32, t[1]);
-          tmem_ld_wait();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_read);
+        tmem_ld_32x32(my_s, t[0]);
+        tmem_ld_32x32(my_s + 32, t[1]);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse),
-                              (e & 7) < kPolyPairs);
-        }
-        const bool masked = j == nblk - 1;  // the diagonal block (causal) and the one in which the document ends
-        if (masked) {
-          const int limit = (p.causal ? min(tile.len, q_idx + 1) : tile.len) - j * 128 - sub * 64;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 v = both(pr[e]);
-            pr[e] = pair(2 * e < limit ? v.x : 0.f, 2 * e + 1 < limit ? v.y : 0.f);
-          }
-        }
+        for (int e = 0; e < 32; ++e)
+          pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse),
+                            (e & 7) < kPolyPairs);
         if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
+        tmem_ld_32x32(my_dp, t[0]);
+        tmem_ld_32x32(my_dp + 32, t[1]);
+        tmem_ld_wait();
+        // dP was the only reader of this V tile; the last one's memory serves the epilogue first
+        if (lane == 0 && j + 1 < nblk) mbar_arrive(&v_empty[n % kStagesV]);
+        // the diagonal block (causal) and the one in which the document ends are masked, in the packed result: what a masked
+        // score gave, Inf or NaN, is gone with it
+        const int limit = j < nblk - 1 ? 64 : (p.causal ? min(tile.len, q_idx + 1) : tile.len) - j * 128 - sub * 64;
+        const bool masked = j == nblk - 1;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t t[32], pk[16];
-          tmem_ld_32x32(my_dp + c * 32, t);
-          tmem_ld_wait();
+          uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float2 d = both(mul2(pr[c * 16 + e], add2(pair(__uint_as_float(t[2 * e]), __uint_as_float(t[2 * e + 1])), minus_delta)));
+            const float2 d = both(mul2(pr[c * 16 + e], add2(pair(__uint_as_float(t[c][2 * e]), __uint_as_float(t[c][2 * e + 1])), minus_delta)));
             pk[e] = pack_bf16(d.x, d.y);
           }
-          if (masked) {  // 0 * (dP - delta) would let an Inf of a masked column through
+          if (masked) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 v = both(pr[c * 16 + e]);
-              pk[e] &= (v.x == 0.f ? 0u : 0xffffu) | (v.y == 0.f ? 0u : 0xffff0000u);
-            }
+            for (int e = 0; e < 16; ++e) pk[e] &= keep_below(limit - 2 * (c * 16 + e));
           }
-          tmem_st_32x16(my_dp + c * 16, pk);  // the first chunk's dS goes over columns of its own
+          tmem_st_32x16(my_dp + c * 16, pk);
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -423,11 +478,20 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (lane == 0) mbar_arrive(ds_ready);
       }
       if (!ok) break;
+      const int first = q0 + quarter * 32;
+      const int sv = (n - 1) % kStagesV;
+      Turn<D> turn;
+      if (p.cs) turn.fetch(p, first, tile.len - first, sub, lane);
       if (!(ok = warp_wait(acc_full, it & 1, abort_flag))) break;
       tc_fence_after_sync();
-      const long long row = (long long)tile.start + q_idx;
-      write_row<D>(tAcc + lane_off, sub, p.scale, p, p.cs ? q_idx : -1, q_idx < tile.len, p.out_a + row * p.out_stride + h * D);
+      uint8_t* stage = sV + sv * TILE_BYTES + (warp - 4) * (32 * D);
+      __nv_bfloat16* dst = p.out_a + ((long long)tile.start + first) * p.out_stride + h * D;
+      if (p.cs) write_rows<D, true>(tAcc + lane_off, sub, p.scale, turn, tile.len - first, stage, lane, dst, p.out_stride);
+      else write_rows<D, false>(tAcc + lane_off, sub, p.scale, turn, tile.len - first, stage, lane, dst, p.out_stride);
       tc_fence_before_sync();
+      fence_proxy_async_smem();  // the tile's next content comes by TMA
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_empty[sv]);
       ++it;
     }
   }
@@ -489,23 +553,24 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   struct Item {
     int start, len, hkv, kv_tile, first, tiles, blocks;
   };
-  auto item_of = [&](int i) {
-    const TileOrder order = tile_order(i, count, p.Hkv, p.head_group);
-    const Tile tile = p.tiles[order.tile_rank];
-    Item w;
-    w.start = tile.start, w.len = tile.len, w.hkv = order.index;
+  Walk walk(p.tiles, count, p.Hkv, p.head_group);
+  auto next_item = [&](Item& w) {
+    Tile tile;
+    if (!walk.next(tile, w.hkv)) return false;
+    w.start = tile.start, w.len = tile.len;
     w.tiles = (tile.len + 127) / 128;
     w.kv_tile = w.tiles - 1 - tile.rank;
     w.first = p.causal ? w.kv_tile : 0;
     w.blocks = tile.pad ? 0 : G * (w.tiles - w.first);
-    return w;
+    return true;
   };
+  Item w;
 
   if (threadIdx.x == 0) {
     mbar_init(k_full, 1);
     mbar_init(k_empty, 1);
     mbar_init(v_full, 1);
-    mbar_init(v_empty, 1);
+    mbar_init(v_empty, 8);
     for (int i = 0; i < kStagesQ; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
@@ -539,12 +604,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t tDK = tmem_base + 384;   // D columns
 
   bool ok = true;
-  Items items(count * p.Hkv);
   int it = 0;  // items with work so far
   int n = 0;   // blocks so far
-  if (warp == 0) {
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+  // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
+  if (warp < 4) {
+    give_registers<72>();
+    if (warp == 0) {
+    while (ok && next_item(w)) {
       if (w.blocks == 0) continue;
       // rows beyond the document stay in their own accumulator rows, which are not written
       if (!(ok = warp_wait(k_empty, (it & 1) ^ 1, abort_flag))) break;
@@ -599,13 +665,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       __syncwarp();
     };
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const int blocks = item_of(i).blocks;
+    while (ok && next_item(w)) {
+      const int blocks = w.blocks;
       if (blocks == 0) continue;
       if (!(ok = wait(k_full, it & 1) && wait(&q_full[n % kStagesQ], (n / kStagesQ) & 1))) break;
       issue_scores(tS, sK, sQ + (n % kStagesQ) * TILE_BYTES, s_full, blocks == 1 ? k_empty : nullptr);
       if (!(ok = wait(v_full, it & 1) && wait(&do_full[n % kStagesDO], (n / kStagesDO) & 1))) break;
-      issue_scores(tDP, sV, sDO + (n % kStagesDO) * TILE_BYTES, dp_full, blocks == 1 ? v_empty : nullptr);
+      issue_scores(tDP, sV, sDO + (n % kStagesDO) * TILE_BYTES, dp_full, nullptr);
       for (int b = 0; b < blocks; ++b, ++n) {
         const bool more = b + 1 < blocks;
         const int m = n + 1;
@@ -619,7 +685,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         if (!(ok = wait(ds_ready, n & 1))) break;
         issue_acc(tDK, tDP, sQ + (n % kStagesQ) * TILE_BYTES, b, &q_empty[n % kStagesQ], more ? nullptr : acc_full);
-        if (more) issue_scores(tDP, sV, sDO + (m % kStagesDO) * TILE_BYTES, dp_full, b + 2 == blocks ? v_empty : nullptr);
+        if (more) issue_scores(tDP, sV, sDO + (m % kStagesDO) * TILE_BYTES, dp_full, nullptr);
       }
       ++it;
     }
@@ -637,8 +703,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         next[4 + u] = in ? -p.delta[(long long)head * p.T + row + x] : 0.f;
       }
     };
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+    while (ok && next_item(w)) {
       if (w.blocks == 0) continue;
       int head = w.hkv * G, blk = w.first;
       fetch(w, head, blk);
@@ -656,10 +721,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (b + 1 < w.blocks) fetch(w, head, blk);
       }
     }
-  } else if (warp == 3) {
+  } else {
     uint32_t q_phases = 0, do_phases = 0;  // of the raw barriers
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+    while (ok && next_item(w)) {
       if (w.blocks == 0) continue;
       const int per_head = w.tiles - w.first, valid = w.len - (w.tiles - 1) * 128;
       if (valid >= 128) {
@@ -677,15 +741,16 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         clear_tail<NCH>(sDO + sd * TILE_BYTES, valid, &do_full[sd], lane);
       }
     }
+    }
   } else {
+    take_registers<216>();
     const int sub = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;  // key row of this thread
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t my_s = tS + lane_off + sub * 64, my_dp = tDP + lane_off + sub * 64;
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2);
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+    while (ok && next_item(w)) {
       const int k0 = w.kv_tile * 128;
       if (w.blocks == 0) {
         const int rows = min(128, w.len - k0);
@@ -699,32 +764,27 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const f32x2* minus_lse = reinterpret_cast<const f32x2*>(s_stat + st * 256 + sub * 64);
         const f32x2* minus_delta = minus_lse + 64;
         if (!(ok = warp_wait(&stat_full[st], (n / kStagesStat) & 1, abort_flag))) break;
+        // what shared memory gives is asked for ahead of the scores: while the products read their operands there at its full
+        // rate, a load takes its time
+        f32x2 pr[32];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(minus_lse + e);
+          pr[e] = l.x, pr[e + 1] = l.y;
+        }
         if (!(ok = warp_wait(s_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        f32x2 pr[32];
-        {
-          uint32_t t[2][32];
-          tmem_ld_32x32(my_s, t[0]);
-          tmem_ld_32x32(my_s + 32, t[1]);
-          tmem_ld_wait();
+        uint32_t t[2][32];
+        tmem_ld_32x32(my_s, t[0]);
+        tmem_ld_32x32(my_s + 32, t[1]);
+        tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(minus_lse + e);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              pr[e + u] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][((e + u) & 15) * 2]), __uint_as_float(t[e >> 4][((e + u) & 15) * 2 + 1])),
-                                         scale2, u == 0 ? l.x : l.y),
-                                    ((e + u) & 7) < kPolyPairs);
-          }
-        }
-        if (p.causal && blk == w.kv_tile) {  // queries before this key
-          const int first = r - sub * 64;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 v = both(pr[e]);
-            pr[e] = pair(2 * e >= first ? v.x : 0.f, 2 * e + 1 >= first ? v.y : 0.f);
-          }
-        }
+        for (int e = 0; e < 32; ++e)
+          pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, pr[e]),
+                            (e & 7) < kPolyPairs);
+        // queries before this key are masked, in the packed results
+        const bool masked = p.causal && blk == w.kv_tile;
+        const int first = r - sub * 64;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
@@ -733,30 +793,47 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const float2 v = both(pr[c * 16 + e]);
             pk[e] = pack_bf16(v.x, v.y);
           }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] &= ~keep_below(first - 2 * (c * 16 + e));
+          }
           tmem_st_32x16(my_s + c * 16, pk);
         }
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
+        f32x2 dl[16];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(minus_delta + e);
+          dl[e] = d.x, dl[e + 1] = d.y;
+        }
         if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
+        tmem_ld_32x32(my_dp, t[0]);
+        tmem_ld_32x32(my_dp + 32, t[1]);
+        tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t t[32], pk[16];
-          tmem_ld_32x32(my_dp + c * 32, t);
-          tmem_ld_wait();
+          uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(minus_delta + c * 16 + e);
+          for (int e = 0; e < 16; ++e) {
+            const float2 v = both(mul2(pr[c * 16 + e], add2(pair(__uint_as_float(t[c][2 * e]), __uint_as_float(t[c][2 * e + 1])), dl[e])));
+            pk[e] = pack_bf16(v.x, v.y);
+          }
+          if (masked) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float2 v = both(mul2(pr[c * 16 + e + u],
-                                         add2(pair(__uint_as_float(t[2 * (e + u)]), __uint_as_float(t[2 * (e + u) + 1])), u == 0 ? d.x : d.y)));
-              pk[e + u] = pack_bf16(v.x, v.y);
-            }
+            for (int e = 0; e < 16; ++e) pk[e] &= ~keep_below(first - 2 * (c * 16 + e));
           }
           tmem_st_32x16(my_dp + c * 16, pk);
+          if (c == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(minus_delta + 16 + e);
+              dl[e] = d.x, dl[e + 1] = d.y;
+            }
+          }
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -768,14 +845,20 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (++blk == w.tiles) blk = w.first;
       }
       if (!ok) break;
+      const int first = k0 + quarter * 32;
+      Turn<D> turn;
+      if (p.cs) turn.fetch(p, first, w.len - first, sub, lane);
       if (!(ok = warp_wait(acc_full, it & 1, abort_flag))) break;
       tc_fence_after_sync();
-      const int k_idx = k0 + r;
-      const long long row = (long long)w.start + k_idx;
-      const bool row_ok = k_idx < w.len;
-      write_row<D>(tDK + lane_off, sub, p.scale, p, p.cs ? k_idx : -1, row_ok, p.out_a + row * p.out_stride + w.hkv * D);
-      write_row<D>(tDV + lane_off, sub, 1.f, p, -1, row_ok, p.out_b + row * p.out_stride + w.hkv * D);
+      const long long at = ((long long)w.start + first) * p.out_stride + w.hkv * D;
+      uint8_t* stage = sV + (warp - 4) * (32 * D);  // V has been read; its next tile is loaded after this
+      if (p.cs) write_rows<D, true>(tDK + lane_off, sub, p.scale, turn, w.len - first, stage, lane, p.out_a + at, p.out_stride);
+      else write_rows<D, false>(tDK + lane_off, sub, p.scale, turn, w.len - first, stage, lane, p.out_a + at, p.out_stride);
+      write_rows<D, false>(tDV + lane_off, sub, 1.f, turn, w.len - first, stage, lane, p.out_b + at, p.out_stride);
       tc_fence_before_sync();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_empty);
       ++it;
     }
   }
@@ -787,7 +870,7 @@ template <int D>
 static int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                       BwdArgs p, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv, cudaStream_t stream) {
   constexpr int TILE = (D / 64) * kChunkBytes;
-  constexpr int SMEM1 = (2 + kStagesK + kStagesV) * TILE + 2048 + 256;
+  constexpr int SMEM1 = (2 + kStagesK + kStagesV) * TILE + 2560 + 256;
   constexpr int SMEM2 = (2 + kStagesQ + kStagesDO) * TILE + kStagesStat * 1024 + 256;
   static_assert(SMEM1 <= 232448 && SMEM2 <= 232448, "one block's shared memory");
   constexpr auto pass1 = packed_dq_kernel<D>;

@@ -52,7 +52,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint8_t* sQ = smem;                 // 2 tiles
   uint8_t* sK = sQ + 2 * TILE_BYTES;  // 2 stages
   uint8_t* sV = sK + 2 * TILE_BYTES;  // 2 stages
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + 2 * TILE_BYTES);
+  uint8_t* sOut = sV + 2 * TILE_BYTES;  // 4 KB for each softmax warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + 32768);
   uint64_t* q_full = bars;        // [tile]
   uint64_t* q_empty = bars + 2;   // [tile]
   uint64_t* k_full = bars + 4;    // [stage]
@@ -78,37 +79,49 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     int pad_rows;         // padding: rows to clear
     bool split;           // two heads with keys of their own (one block each)
   };
-  auto item_of = [&](int i) {
-    Item w;
-    int entry;
-    bool two_heads = false;
+  // as Walk (attention_packed.cuh): the next item's table entry is on its way while one is worked on
+  Items items(n_wide * p.Hq + (n_docs - n_wide) * head_pairs + (n_all - n_docs) * p.Hq);
+  int next_i, next_head;
+  bool next_pair;
+  Tile next_tile;
+  auto fetch = [&]() {
+    int i = next_i = items.next(), entry;
+    if (i < 0) return;
+    next_pair = false;
     if (i < n_wide * p.Hq) {
       const TileOrder order = tile_order(i, n_wide, p.Hq, p.head_group);
       entry = order.tile_rank;
-      w.head[0] = w.head[1] = order.index;
+      next_head = order.index;
     } else if ((i -= n_wide * p.Hq) < (n_docs - n_wide) * head_pairs) {
       entry = i / head_pairs;
-      w.head[0] = 2 * (i - entry * head_pairs), w.head[1] = w.head[0] + 1;
+      next_head = 2 * (i - entry * head_pairs);
       entry += n_wide;
-      two_heads = true;
+      next_pair = true;
     } else {
       i -= (n_docs - n_wide) * head_pairs;
       entry = i / p.Hq;
-      w.head[0] = w.head[1] = i - entry * p.Hq;
+      next_head = i - entry * p.Hq;
       entry += n_docs;
     }
-    const Tile tile = p.tiles[entry];
+    next_tile = p.tiles[entry];
+  };
+  auto next_item = [&](Item& w) {
+    if (next_i < 0) return false;
+    const Tile tile = next_tile;
     w.start = tile.start, w.len = tile.len;
-    w.row[0] = tile.rank * 256, w.row[1] = two_heads ? w.row[0] : w.row[0] + 128;
+    w.head[0] = next_head, w.head[1] = next_pair ? next_head + 1 : next_head;
+    w.row[0] = tile.rank * 256, w.row[1] = next_pair ? w.row[0] : w.row[0] + 128;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
       w.blocks[t] = tile.pad || w.row[t] >= tile.len || w.head[t] >= p.Hq
                         ? 0 : ((p.causal ? min(tile.len, w.row[t] + 128) : tile.len) + 127) / 128;
-    w.split = w.blocks[1] > 0 && w.head[0] / G != w.head[1] / G;
+    w.split = next_pair && w.blocks[1] > 0 && w.head[0] / G != w.head[1] / G;
     w.pad_rows = tile.pad ? min(256, tile.len - w.row[0]) : 0;
-    return w;
+    fetch();
+    return true;
   };
-  Items items(n_wide * p.Hq + (n_docs - n_wide) * head_pairs + (n_all - n_docs) * p.Hq);
+  fetch();
+  Item w;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -135,9 +148,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   bool ok = true;
   int used[2] = {0, 0};  // items so far that had the tile
   int n = 0;             // K / V stages so far
-  if (warp == 0) {
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+  // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
+  if (warp < 4) {
+    give_registers<72>();
+    if (warp == 0) {
+    while (ok && next_item(w)) {
       if (w.blocks[0] == 0) continue;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -196,8 +211,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __syncwarp();
     };
     int done[2] = {0, 0};  // blocks so far, by tile
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+    while (ok && next_item(w)) {
       if (w.blocks[0] == 0) continue;
       // stage of block j of a tile, and whether the tile is the last to read it
       auto stage_of = [&](int t, int j) { return n + j + (w.split ? t : 0); };
@@ -230,8 +244,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the v_raw barriers
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+    while (ok && next_item(w)) {
       if (w.blocks[0] == 0) continue;
       const int nblk = max(w.blocks[0], w.blocks[1]), stages = w.split ? 2 : nblk;
       const int valid = w.len - (nblk - 1) * 128;  // only the last block can reach beyond the document
@@ -243,7 +256,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       n += stages;
     }
-  } else if (warp >= 4) {
+    }
+  } else {
+    take_registers<216>();
     // ------------------------------------------------------------ softmax + epilogue, one query row per thread
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
@@ -253,8 +268,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2);
     int done = 0;  // blocks so far
     int mine = 0;  // items so far
-    for (int i; ok && (i = items.next()) >= 0;) {
-      const Item w = item_of(i);
+    while (ok && next_item(w)) {
       if (w.pad_rows > 0) {
         clear_rows<D>(p.o, p.o_stride, (long long)w.start + w.row[0], w.pad_rows, w.head[0] * D, threadIdx.x - 128, 256);
         continue;
@@ -348,26 +362,36 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_after_sync();
       const float2 lb = both(l2);
       const float l = lb.x + lb.y, inv_l = 1.f / l;
-      const long long row = (long long)w.start + q_idx;
+      // through memory of the warp's own, 128-byte pieces of 32 rows at a time: whole lines leave (see write_rows in
+      // attention_packed_bwd.cu)
+      const int first = first_row + quarter * 32;
+      __nv_bfloat16* dst = p.o + ((long long)w.start + first) * p.o_stride + h * D;
+      uint8_t* stage = sOut + (warp - 4) * 4096;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32(tO + c * 32, o);
+      for (int c = 0; c < NCH; ++c) {
+        uint32_t o[2][32];
+        tmem_ld_32x32(tO + c * 64, o[0]);
+        tmem_ld_32x32(tO + c * 64 + 32, o[1]);
         tmem_ld_wait();
-        if (q_idx < w.len) {
-          __nv_bfloat16* dst = p.o + row * p.o_stride + h * D + c * 32;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t b[4];
+        for (int u = 0; u < 8; ++u) {
+          uint32_t b[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              b[e] = pack_bf16(__uint_as_float(o[u * 8 + e * 2]) * inv_l, __uint_as_float(o[u * 8 + e * 2 + 1]) * inv_l);
-            reinterpret_cast<uint4*>(dst)[u] = make_uint4(b[0], b[1], b[2], b[3]);
-          }
+          for (int e = 0; e < 4; ++e)
+            b[e] = pack_bf16(__uint_as_float(o[u >> 2][(u & 3) * 8 + e * 2]) * inv_l,
+                             __uint_as_float(o[u >> 2][(u & 3) * 8 + e * 2 + 1]) * inv_l);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
         }
-        __syncwarp();  // the next load of TMEM is one of the whole warp
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = k * 4 + (lane >> 3), u = lane & 7;
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+          if (first + r < w.len) *reinterpret_cast<uint4*>(dst + r * p.o_stride + c * 64 + u * 8) = x;
+        }
+        __syncwarp();
       }
-      if (q_idx < w.len) p.lse[(long long)h * p.T + row] = (m + log2f(l)) * 0.6931471805599453f;
+      if (q_idx < w.len) p.lse[(long long)h * p.T + w.start + q_idx] = (m + log2f(l)) * 0.6931471805599453f;
       tc_fence_before_sync();
     }
   }
@@ -378,7 +402,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 template <int D>
 static int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdArgs& p, int max_tiles,
                       cudaStream_t stream) {
-  constexpr int SMEM = 6 * (D / 64) * kChunkBytes + 256;
+  constexpr int SMEM = 6 * (D / 64) * kChunkBytes + 32768 + 256;
   constexpr auto kern = packed_fwd_kernel<D>;
   if (cudaError_t e = pb::allow_smem<kern, SMEM>(); e != cudaSuccess) return (int)e;
   kern<<<resident_blocks((long long)max_tiles * p.Hq), kFwdThreads, SMEM, stream>>>(tq, tk, tv, p);
