@@ -165,29 +165,38 @@ __device__ __forceinline__ void leave(volatile int* abort_flag, int warp, uint32
   if (warp == 1) tmem_dealloc<1>(tmem_base, 512);
 }
 
-// Items of a table of tiles and heads (tile_order), with the next one's table entry on its way while one is worked on: the
-// read of the table took 1 000 cycles between two items.
-struct Walk {
-  Items items;
-  const Tile* tiles;
-  int count, heads, group;
-  int i, head;
-  Tile tile;
-  __device__ __forceinline__ Walk(const Tile* tiles, int count, int heads, int group)
-      : items(count * heads), tiles(tiles), count(count), heads(heads), group(group) {
-    fetch();
+// The loading warp decodes an item (a read of the table, three divisions: 1 000 cycles and more) ahead of the others and hands it
+// on through shared memory; they take 100 cycles to get it.
+struct ItemRing {
+  static constexpr int kDepth = 4, kBytes = kDepth * 48, kBars = 2 * kDepth;
+  int4* data;  // [kDepth][3]
+  uint64_t *full, *empty;
+  int n = 0;
+  __device__ __forceinline__ ItemRing(uint8_t* mem, uint64_t* bars)
+      : data(reinterpret_cast<int4*>(mem)), full(bars), empty(bars + kDepth) {}
+  __device__ __forceinline__ void init(int readers) {
+    for (int i = 0; i < kDepth; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], readers);
+    }
   }
-  __device__ __forceinline__ void fetch() {
-    if ((i = items.next()) < 0) return;
-    const TileOrder order = tile_order(i, count, heads, group);
-    head = order.index;
-    tile = tiles[order.tile_rank];
+  __device__ __forceinline__ bool put(int4 a, int4 b, int4 c, int lane, volatile int* abort_flag) {
+    const int s = n % kDepth;
+    if (!warp_wait(&empty[s], ((n / kDepth) & 1) ^ 1, abort_flag)) return false;
+    if (lane == 0) {
+      data[s * 3] = a, data[s * 3 + 1] = b, data[s * 3 + 2] = c;
+      mbar_arrive(&full[s]);
+    }
+    ++n;
+    return true;
   }
-  __device__ __forceinline__ bool next(Tile& t, int& h) {
-    if (i < 0) return false;
-    t = tile;
-    h = head;
-    fetch();
+  __device__ __forceinline__ bool get(int4& a, int4& b, int4& c, int lane, volatile int* abort_flag) {
+    const int s = n % kDepth;
+    if (!warp_wait(&full[s], (n / kDepth) & 1, abort_flag)) return false;
+    a = data[s * 3], b = data[s * 3 + 1], c = data[s * 3 + 2];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[s]);
+    ++n;
     return true;
   }
 };

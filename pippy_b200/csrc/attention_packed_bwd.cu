@@ -189,15 +189,36 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_ready = s_full + 3;
   uint64_t* acc_full = s_full + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5);
+  ItemRing ring(reinterpret_cast<uint8_t*>(bars) + 256, s_full + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5 + ItemRing::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int count = *p.count;
   const int G = p.Hq / p.Hkv;
-  auto blocks_of = [&](const Tile& t) {
-    return t.pad ? 0 : ((p.causal ? min(t.len, t.rank * 128 + 128) : t.len) + 127) / 128;
+  // an item: a tile of queries of head h and the blocks of keys that it sees (0: padding)
+  Items items(count * p.Hq);
+  bool ok = true;
+  Tile tile;
+  int h = 0, nblk = 0;
+  auto publish_next = [&]() {  // by the loading warp; false after the last
+    const int i = items.next();
+    tile.start = -1;
+    if (i >= 0) {
+      const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
+      tile = p.tiles[order.tile_rank];
+      h = order.index;
+      nblk = tile.pad ? 0 : ((p.causal ? min(tile.len, tile.rank * 128 + 128) : tile.len) + 127) / 128;
+    }
+    ok = ring.put(make_int4(tile.start, tile.len, tile.rank, h), make_int4(nblk, 0, 0, 0), make_int4(0, 0, 0, 0), lane, abort_flag);
+    return ok && tile.start >= 0;
+  };
+  auto next_item = [&]() {  // by the others
+    int4 a, b, c;
+    if (!(ok = ring.get(a, b, c, lane, abort_flag))) return false;
+    tile.start = a.x, tile.len = a.y, tile.rank = a.z, h = a.w, nblk = b.x;
+    return tile.start >= 0;
   };
 
   if (threadIdx.x == 0) {
@@ -219,6 +240,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 8);
     mbar_init(acc_full, 1);
+    ring.init(14);  // MMA, clearing, softmax, Q and dO
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -233,18 +255,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t tDP = tmem_base + 256;   // 128 columns; dS over them
   const uint32_t tAcc = tmem_base + 384;  // D columns
 
-  bool ok = true;
-  Walk walk(p.tiles, count, p.Hq, p.head_group);
-  Tile tile;
-  int h;
   int it = 0;  // items with work so far
   int n = 0;   // blocks so far
   // launched with 128 registers a thread: 64 + 2 x 168 + 112 = 4 x 128
   if (warp < 4) {
     give_registers<64>();
     if (warp == 0) {
-    while (ok && walk.next(tile, h)) {
-      const int nblk = blocks_of(tile);
+    while (ok && publish_next()) {
       if (nblk == 0) continue;
       const int hkv = h / G;
       if (!(ok = warp_wait(stage_empty, (it & 1) ^ 1, abort_flag))) break;
@@ -289,8 +306,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       __syncwarp();
     };
-    while (ok && walk.next(tile, h)) {
-      const int nblk = blocks_of(tile);
+    while (ok && next_item()) {
       if (nblk == 0) continue;
       if (!(ok = wait(res_ready, it & 1) && wait(&k_full[n % kStagesK], (n / kStagesK) & 1))) break;
       issue_scores(tS, tQ, sK + (n % kStagesK) * TILE_BYTES, s_full, nullptr);
@@ -322,8 +338,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the k_raw barriers
-    while (ok && walk.next(tile, h)) {
-      const int nblk = blocks_of(tile);
+    while (ok && next_item()) {
       if (nblk == 0) continue;
       n += nblk;
       const int valid = tile.len - (nblk - 1) * 128;  // only an item's last block can reach beyond its document
@@ -339,8 +354,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    while (ok && walk.next(tile, h)) {
-      if (blocks_of(tile) == 0) continue;
+    while (ok && next_item()) {
+      if (nblk == 0) continue;
       const bool row_ok = tile.rank * 128 + r < tile.len;
       const long long row = (long long)tile.start + tile.rank * 128 + r;
       const float lse2 = row_ok ? p.lse[(long long)h * p.T + row] * kLog2e : 0.f;
@@ -420,8 +435,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t my_s = tS + lane_off + sub * 64, my_dp = tDP + lane_off + sub * 64;
-    while (ok && walk.next(tile, h)) {
-      const int nblk = blocks_of(tile);
+    while (ok && next_item()) {
       const int q0 = tile.rank * 128, q_idx = q0 + r;
       if (nblk == 0) {
         clear_rows<D>(p.out_a, p.out_stride, (long long)tile.start + q0, min(128, tile.len - q0), h * D, threadIdx.x - 128, 256);
@@ -541,7 +555,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_ready = s_full + 3;
   uint64_t* acc_full = s_full + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5);
+  ItemRing ring(reinterpret_cast<uint8_t*>(bars) + 320, s_full + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5 + ItemRing::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -553,18 +568,32 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   struct Item {
     int start, len, hkv, kv_tile, first, tiles, blocks;
   };
-  Walk walk(p.tiles, count, p.Hkv, p.head_group);
-  auto next_item = [&](Item& w) {
-    Tile tile;
-    if (!walk.next(tile, w.hkv)) return false;
-    w.start = tile.start, w.len = tile.len;
+  Items items(count * p.Hkv);
+  bool ok = true;
+  Item w;
+  auto decode = [&](int i) {
+    const TileOrder order = tile_order(i, count, p.Hkv, p.head_group);
+    const Tile tile = p.tiles[order.tile_rank];
+    w.start = tile.start, w.len = tile.len, w.hkv = order.index;
     w.tiles = (tile.len + 127) / 128;
     w.kv_tile = w.tiles - 1 - tile.rank;
     w.first = p.causal ? w.kv_tile : 0;
     w.blocks = tile.pad ? 0 : G * (w.tiles - w.first);
-    return true;
   };
-  Item w;
+  auto publish_next = [&]() {  // by the loading warp; false after the last
+    const int i = items.next();
+    w.start = -1;
+    if (i >= 0) decode(i);
+    ok = ring.put(make_int4(w.start, w.len, w.hkv, w.kv_tile), make_int4(w.first, w.tiles, w.blocks, 0), make_int4(0, 0, 0, 0), lane, abort_flag);
+    return ok && w.start >= 0;
+  };
+  auto next_item = [&]() {  // by the others
+    int4 a, b, c;
+    if (!(ok = ring.get(a, b, c, lane, abort_flag))) return false;
+    w.start = a.x, w.len = a.y, w.hkv = a.z, w.kv_tile = a.w;
+    w.first = b.x, w.tiles = b.y, w.blocks = b.z;
+    return w.start >= 0;
+  };
 
   if (threadIdx.x == 0) {
     mbar_init(k_full, 1);
@@ -590,6 +619,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 8);
     mbar_init(acc_full, 1);
+    ring.init(11);  // MMA, lse and delta, clearing, softmax
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -603,14 +633,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t tDV = tmem_base + 256;   // D columns
   const uint32_t tDK = tmem_base + 384;   // D columns
 
-  bool ok = true;
   int it = 0;  // items with work so far
   int n = 0;   // blocks so far
   // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
   if (warp < 4) {
     give_registers<72>();
     if (warp == 0) {
-    while (ok && next_item(w)) {
+    while (ok && publish_next()) {
       if (w.blocks == 0) continue;
       // rows beyond the document stay in their own accumulator rows, which are not written
       if (!(ok = warp_wait(k_empty, (it & 1) ^ 1, abort_flag))) break;
@@ -665,7 +694,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       __syncwarp();
     };
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       const int blocks = w.blocks;
       if (blocks == 0) continue;
       if (!(ok = wait(k_full, it & 1) && wait(&q_full[n % kStagesQ], (n / kStagesQ) & 1))) break;
@@ -703,7 +732,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         next[4 + u] = in ? -p.delta[(long long)head * p.T + row + x] : 0.f;
       }
     };
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       if (w.blocks == 0) continue;
       int head = w.hkv * G, blk = w.first;
       fetch(w, head, blk);
@@ -723,7 +752,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
   } else {
     uint32_t q_phases = 0, do_phases = 0;  // of the raw barriers
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       if (w.blocks == 0) continue;
       const int per_head = w.tiles - w.first, valid = w.len - (w.tiles - 1) * 128;
       if (valid >= 128) {
@@ -750,7 +779,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t my_s = tS + lane_off + sub * 64, my_dp = tDP + lane_off + sub * 64;
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2);
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       const int k0 = w.kv_tile * 128;
       if (w.blocks == 0) {
         const int rows = min(128, w.len - k0);
@@ -870,8 +899,8 @@ template <int D>
 static int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                       BwdArgs p, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv, cudaStream_t stream) {
   constexpr int TILE = (D / 64) * kChunkBytes;
-  constexpr int SMEM1 = (2 + kStagesK + kStagesV) * TILE + 2560 + 256;
-  constexpr int SMEM2 = (2 + kStagesQ + kStagesDO) * TILE + kStagesStat * 1024 + 256;
+  constexpr int SMEM1 = (2 + kStagesK + kStagesV) * TILE + 2560 + 256 + ItemRing::kBytes;
+  constexpr int SMEM2 = (2 + kStagesQ + kStagesDO) * TILE + kStagesStat * 1024 + 320 + ItemRing::kBytes;
   static_assert(SMEM1 <= 232448 && SMEM2 <= 232448, "one block's shared memory");
   constexpr auto pass1 = packed_dq_kernel<D>;
   constexpr auto pass2 = packed_dkv_kernel<D>;

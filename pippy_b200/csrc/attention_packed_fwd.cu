@@ -64,7 +64,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* s_full = bars + 14;   // [tile]
   uint64_t* p_ready = bars + 16;  // [tile]
   uint64_t* o_full = bars + 18;   // [tile]: the item's last P V
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  ItemRing ring(sOut + 32768 + 256, bars + 20);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20 + ItemRing::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -79,49 +80,56 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     int pad_rows;         // padding: rows to clear
     bool split;           // two heads with keys of their own (one block each)
   };
-  // as Walk (attention_packed.cuh): the next item's table entry is on its way while one is worked on
+  // decoded by the loading warp, taken from the ring by the others; false after the last
   Items items(n_wide * p.Hq + (n_docs - n_wide) * head_pairs + (n_all - n_docs) * p.Hq);
-  int next_i, next_head;
-  bool next_pair;
-  Tile next_tile;
-  auto fetch = [&]() {
-    int i = next_i = items.next(), entry;
-    if (i < 0) return;
-    next_pair = false;
+  bool ok = true;
+  Item w;
+  auto decode = [&]() {
+    int i = items.next(), entry;
+    if (i < 0) {
+      w.start = -1;
+      return;
+    }
+    bool two_heads = false;
     if (i < n_wide * p.Hq) {
       const TileOrder order = tile_order(i, n_wide, p.Hq, p.head_group);
       entry = order.tile_rank;
-      next_head = order.index;
+      w.head[0] = w.head[1] = order.index;
     } else if ((i -= n_wide * p.Hq) < (n_docs - n_wide) * head_pairs) {
       entry = i / head_pairs;
-      next_head = 2 * (i - entry * head_pairs);
+      w.head[0] = 2 * (i - entry * head_pairs), w.head[1] = w.head[0] + 1;
       entry += n_wide;
-      next_pair = true;
+      two_heads = true;
     } else {
       i -= (n_docs - n_wide) * head_pairs;
       entry = i / p.Hq;
-      next_head = i - entry * p.Hq;
+      w.head[0] = w.head[1] = i - entry * p.Hq;
       entry += n_docs;
     }
-    next_tile = p.tiles[entry];
-  };
-  auto next_item = [&](Item& w) {
-    if (next_i < 0) return false;
-    const Tile tile = next_tile;
+    const Tile tile = p.tiles[entry];
     w.start = tile.start, w.len = tile.len;
-    w.head[0] = next_head, w.head[1] = next_pair ? next_head + 1 : next_head;
-    w.row[0] = tile.rank * 256, w.row[1] = next_pair ? w.row[0] : w.row[0] + 128;
+    w.row[0] = tile.rank * 256, w.row[1] = two_heads ? w.row[0] : w.row[0] + 128;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
       w.blocks[t] = tile.pad || w.row[t] >= tile.len || w.head[t] >= p.Hq
                         ? 0 : ((p.causal ? min(tile.len, w.row[t] + 128) : tile.len) + 127) / 128;
-    w.split = next_pair && w.blocks[1] > 0 && w.head[0] / G != w.head[1] / G;
+    w.split = two_heads && w.blocks[1] > 0 && w.head[0] / G != w.head[1] / G;
     w.pad_rows = tile.pad ? min(256, tile.len - w.row[0]) : 0;
-    fetch();
-    return true;
   };
-  fetch();
-  Item w;
+  auto publish_next = [&]() {
+    decode();
+    ok = ring.put(make_int4(w.start, w.len, w.row[0], w.row[1]), make_int4(w.head[0], w.head[1], w.blocks[0], w.blocks[1]),
+                  make_int4(w.split, w.pad_rows, 0, 0), lane, abort_flag);
+    return ok && w.start >= 0;
+  };
+  auto next_item = [&]() {
+    int4 a, b, c;
+    if (!(ok = ring.get(a, b, c, lane, abort_flag))) return false;
+    w.start = a.x, w.len = a.y, w.row[0] = a.z, w.row[1] = a.w;
+    w.head[0] = b.x, w.head[1] = b.y, w.blocks[0] = b.z, w.blocks[1] = b.w;
+    w.split = c.x, w.pad_rows = c.y;
+    return w.start >= 0;
+  };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -136,6 +144,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       mbar_init(&p_ready[i], 4);
       mbar_init(&o_full[i], 1);
     }
+    ring.init(10);  // MMA, clearing, softmax
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -145,14 +154,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;  // S/P of tile t: columns [128 t, 128 t + 128); O: [256 + 128 t, + D)
 
-  bool ok = true;
   int used[2] = {0, 0};  // items so far that had the tile
   int n = 0;             // K / V stages so far
   // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
   if (warp < 4) {
     give_registers<72>();
     if (warp == 0) {
-    while (ok && next_item(w)) {
+    while (ok && publish_next()) {
       if (w.blocks[0] == 0) continue;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -211,7 +219,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __syncwarp();
     };
     int done[2] = {0, 0};  // blocks so far, by tile
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       if (w.blocks[0] == 0) continue;
       // stage of block j of a tile, and whether the tile is the last to read it
       auto stage_of = [&](int t, int j) { return n + j + (w.split ? t : 0); };
@@ -244,7 +252,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the v_raw barriers
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       if (w.blocks[0] == 0) continue;
       const int nblk = max(w.blocks[0], w.blocks[1]), stages = w.split ? 2 : nblk;
       const int valid = w.len - (nblk - 1) * 128;  // only the last block can reach beyond the document
@@ -268,7 +276,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2);
     int done = 0;  // blocks so far
     int mine = 0;  // items so far
-    while (ok && next_item(w)) {
+    while (ok && next_item()) {
       if (w.pad_rows > 0) {
         clear_rows<D>(p.o, p.o_stride, (long long)w.start + w.row[0], w.pad_rows, w.head[0] * D, threadIdx.x - 128, 256);
         continue;
@@ -402,7 +410,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 template <int D>
 static int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdArgs& p, int max_tiles,
                       cudaStream_t stream) {
-  constexpr int SMEM = 6 * (D / 64) * kChunkBytes + 32768 + 256;
+  constexpr int SMEM = 6 * (D / 64) * kChunkBytes + 32768 + 256 + ItemRing::kBytes;
   constexpr auto kern = packed_fwd_kernel<D>;
   if (cudaError_t e = pb::allow_smem<kern, SMEM>(); e != cudaSuccess) return (int)e;
   kern<<<resident_blocks((long long)max_tiles * p.Hq), kFwdThreads, SMEM, stream>>>(tq, tk, tv, p);

@@ -31,9 +31,18 @@ def _use_kernels(*tensors: torch.Tensor) -> bool:
 
 def _on_device_of(t: torch.Tensor):
     """Launches go to the current device's stream: makes ``t``'s device the current one where it is not."""
-    if not t.is_cuda or t.device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
+    if t.device.index == torch._C._cuda_getDevice():
+        return _NOWHERE_ELSE
     return torch.cuda.device(t.device)
+
+
+_NOWHERE_ELSE = contextlib.nullcontext()
+
+
+def _no_second_derivative(what: str) -> None:
+    """In a backward: gradients are only recorded there when the caller asked for a graph of them."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative on the kernel path")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -596,8 +605,8 @@ class _SortedEmbeddingFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _no_second_derivative("embedding with sorted gradients")
         ids, positions = ctx.saved_tensors
         wte, wpe = ctx.params
         S, scale = ctx.cfg
@@ -687,18 +696,26 @@ class PackedLayout:
 
     ``positions``: int32 ``[rows * tokens_per_row]``, each token's place in its document, -1 in padding."""
 
-    def __init__(self, lengths: torch.Tensor, tokens_per_row: int, positions: torch.Tensor):
+    def __init__(self, lengths: torch.Tensor, tokens_per_row: int, positions: torch.Tensor, tables=None, most=(0, 0)):
         self.lengths, self.tokens_per_row, self.positions = lengths, tokens_per_row, positions
         self.rows = lengths.shape[0]
+        self.total = self.rows * tokens_per_row
         self.device = lengths.device
-        # kernel path: tile tables by rows per tile, the most entries they can have, and their used lengths
-        self.tiles: dict = {}
-        self.max_tiles: dict = {}
-        self.counts: dict = {}
+        # kernel path: the tiles of 128 and of 256 rows (4 ints each, room for `most` of them), then for both tables 4 ints:
+        # how many there are, how many before the half-filled ones, how many before the padding
+        self._tables, self._most = tables, most
 
-    @property
-    def total(self) -> int:
-        return self.rows * self.tokens_per_row
+    def tiles(self, rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``(tiles, counts)`` of ``rows`` = 128 or 256 rows, for inspection: ``[n, 4]`` of document start, document
+        length, number of the tile in it, 1 for padding."""
+        first, n = (0, self._most[0]) if rows == 128 else (self._most[0], self._most[1])
+        counts = self._tables[4 * sum(self._most) :].view(2, 4)[0 if rows == 128 else 1]
+        return self._tables[4 * first : 4 * (first + n)].view(n, 4), counts
+
+    def _addresses(self):
+        """Addresses of the tiles of 128 and of 256 rows and of their counts."""
+        base, (n128, n256) = self._tables.data_ptr(), self._most
+        return base, base + 16 * n128, base + 16 * (n128 + n256), base + 16 * (n128 + n256) + 16
 
 
 def packed_layout(lengths: torch.Tensor, tokens_per_row: int) -> PackedLayout:
@@ -733,18 +750,16 @@ def packed_layout(lengths: torch.Tensor, tokens_per_row: int) -> PackedLayout:
         # lengths beyond 32 bits would wrap to ones that seem to fit
         given = (lengths if lengths.dtype == torch.int32 else lengths.clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
         segments = rows * (docs + 1)
-        most = {n: rows * S // n + min(segments, rows * S) for n in (128, 256)}
-        # one buffer, every part on a 16-byte boundary: tiles of 4 ints, then segments, counts, positions
-        ints = 4 * (most[128] + most[256]), (2 * segments + 3) // 4 * 4, 8
-        buf = torch.empty(sum(ints) + rows * S, dtype=torch.int32, device=lengths.device)
-        tiles, segs, counts, positions = buf.split([*ints, rows * S])
-        layout = PackedLayout(given, S, positions)
-        layout.tiles = {128: tiles[: 4 * most[128]], 256: tiles[4 * most[128]:]}
-        layout.max_tiles, layout.counts = most, {128: counts[:4], 256: counts[4:]}
+        spare = min(segments, rows * S)
+        n128, n256 = rows * S // 128 + spare, rows * S // 256 + spare
+        # one buffer: tiles of 4 ints, counts, segments of 2 ints (an even number of them), positions
+        first = 4 * (n128 + n256) + 8 + (2 * segments + 3) // 4 * 4
+        buf = torch.empty(first + rows * S, dtype=torch.int32, device=lengths.device)
+        layout = PackedLayout(given, S, buf[first:], buf[: 4 * (n128 + n256) + 8], (n128, n256))
+        t128, t256, counts, _ = layout._addresses()
         _lib.check(
-            _lib.lib().pb_packed_layout(_lib.addr(given), rows, docs, S, _lib.addr(positions), _lib.addr(segs),
-                                        _lib.addr(layout.tiles[128]), most[128], _lib.addr(layout.tiles[256]), most[256],
-                                        _lib.addr(counts), _lib.err_addr(lengths.device), _lib.stream_addr()),
+            _lib.lib().pb_packed_layout(given.data_ptr(), rows, docs, S, t128 + 4 * first, counts + 32, t128, n128, t256,
+                                        n256, counts, _lib.err_addr(lengths.device), _lib.stream_addr()),
             "pb_packed_layout",
         )
     return layout
@@ -756,59 +771,58 @@ class _PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, cos, sin, layout, Hq, Hkv, D, scale, causal, inplace):
+        # q, k and v are columns of qkv (of qk): addresses instead of views, which cost more than the launch in small calls
         T, nq, nk = layout.total, Hq * D, Hkv * D
         lib, err = _lib.lib(), _lib.err_addr(qkv.device)
         with _on_device_of(qkv):
+            stream = _lib.stream_addr()
             qk = qkv
             if cos is not None:
                 if not inplace:
                     qk = torch.empty(T, nq + nk, device=qkv.device, dtype=qkv.dtype)
                 _lib.check(
-                    lib.pb_packed_rope(_lib.addr(qkv), qkv.stride(0), _lib.addr(qk), qk.stride(0), _lib.addr(cos),
-                                       _lib.addr(sin), _lib.addr(layout.positions), T, Hq + Hkv, D, cos.shape[0], err,
-                                       _lib.stream_addr()),
+                    lib.pb_packed_rope(qkv.data_ptr(), qkv.stride(0), qk.data_ptr(), qk.stride(0), cos.data_ptr(),
+                                       sin.data_ptr(), layout.positions.data_ptr(), T, Hq + Hkv, D, cos.shape[0], err,
+                                       stream),
                     "pb_packed_rope",
                 )
                 if inplace:
                     torch.autograd.graph.increment_version(qkv)
-            q, k, v = qk[:, :nq], qk[:, nq : nq + nk], qkv[:, nq + nk :]
             o = torch.empty(T, nq, device=qkv.device, dtype=qkv.dtype)
             lse = torch.empty(Hq, T, device=qkv.device, dtype=torch.float32)
+            _, t256, _, counts = layout._addresses()
+            q, v, pitch = qk.data_ptr(), qkv.data_ptr() + 2 * (nq + nk), qk.stride(0)
             _lib.check(
-                lib.pb_packed_attention_fwd(_lib.addr(q), _lib.addr(k), _lib.addr(v), _lib.addr(o), _lib.addr(lse),
-                                            _lib.addr(layout.tiles[256]), _lib.addr(layout.counts[256]),
-                                            layout.max_tiles[256], T, Hq, Hkv, D, qk.stride(0), qk.stride(0),
-                                            qkv.stride(0), o.stride(0), scale, int(causal), err, _lib.stream_addr()),
+                lib.pb_packed_attention_fwd(q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), t256, counts,
+                                            layout._most[1], T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, scale,
+                                            int(causal), err, stream),
                 "pb_packed_attention_fwd",
             )
         ctx.save_for_backward(qkv, qk, o, lse, cos, sin)
-        ctx.layout = layout
-        ctx.cfg = (Hq, Hkv, D, scale, causal)
+        ctx.cfg = (layout, Hq, Hkv, D, scale, causal)
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
+        _no_second_derivative("packed_attention")
         qkv, qk, o, lse, cos, sin = ctx.saved_tensors
-        layout = ctx.layout
-        Hq, Hkv, D, scale, causal = ctx.cfg
+        layout, Hq, Hkv, D, scale, causal = ctx.cfg
         T, nq, nk = layout.total, Hq * D, Hkv * D
         with _on_device_of(qkv):
             do = _aligned(do)
-            q, k, v = qk[:, :nq], qk[:, nq : nq + nk], qkv[:, nq + nk :]
             dqkv = torch.empty(T, nq + 2 * nk, device=qkv.device, dtype=qkv.dtype)
-            dq, dk, dv = dqkv[:, :nq], dqkv[:, nq : nq + nk], dqkv[:, nq + nk :]
             delta = torch.empty(Hq, T, device=qkv.device, dtype=torch.float32)
+            t128, _, counts, _ = layout._addresses()
+            q, v, d, pitch = qk.data_ptr(), qkv.data_ptr() + 2 * (nq + nk), dqkv.data_ptr(), qk.stride(0)
             _lib.check(
                 _lib.lib().pb_packed_attention_bwd(
-                    _lib.addr(do), _lib.addr(q), _lib.addr(k), _lib.addr(v), _lib.addr(o), _lib.addr(lse),
-                    _lib.addr(delta), _lib.addr(dq), _lib.addr(dk), _lib.addr(dv), _lib.addr(cos), _lib.addr(sin),
-                    0 if cos is None else cos.shape[0], _lib.addr(layout.tiles[128]), _lib.addr(layout.counts[128]),
-                    layout.max_tiles[128], T, Hq, Hkv, D, qk.stride(0), qk.stride(0), qkv.stride(0), o.stride(0),
-                    do.stride(0), dqkv.stride(0), scale, int(causal), _lib.err_addr(qkv.device), _lib.stream_addr()),
+                    do.data_ptr(), q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), delta.data_ptr(), d, d + 2 * nq,
+                    d + 2 * (nq + nk), _lib.addr(cos), _lib.addr(sin), 0 if cos is None else cos.shape[0], t128, counts,
+                    layout._most[0], T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, nq, nq + 2 * nk, scale, int(causal),
+                    _lib.err_addr(qkv.device), _lib.stream_addr()),
                 "pb_packed_attention_bwd",
             )
-        return (dqkv,) + (None,) * 9
+        return dqkv, None, None, None, None, None, None, None, None, None
 
 
 def packed_attention(qkv, cos, sin, layout: PackedLayout, Hq: int, Hkv: int, D: int, scale: Optional[float] = None,
@@ -899,27 +913,32 @@ class _DropoutFn(torch.autograd.Function):
     def forward(ctx, x, residual, seed, seed_value: int, stream: int, threshold: int):
         ctx.save_for_backward(seed)
         ctx.cfg = (seed_value, stream, threshold)
-        return _DropoutFn.launch(x, residual, seed, seed_value, stream, threshold)
+        return _launch_dropout(x, residual, seed, seed_value, stream, threshold)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         (seed,) = ctx.saved_tensors
-        dx = _DropoutFn.launch(dy, None, seed, *ctx.cfg) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            if torch.is_grad_enabled():  # linear in dy: its derivative is the same mask once more
+                dx = _DropoutFn.apply(dy, None, seed, *ctx.cfg)
+            else:
+                dx = _launch_dropout(dy, None, seed, *ctx.cfg)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
 
-    @staticmethod
-    def launch(x, residual, seed, seed_value, stream, threshold):
-        x = x.contiguous()
-        residual = None if residual is None else residual.contiguous()
-        y = torch.empty_like(x)
-        with _on_device_of(x):
-            _lib.check(
-                _lib.lib().pb_dropout(_lib.addr(x), _lib.addr(residual), _lib.addr(y), x.numel(), _lib.addr(seed),
-                                      seed_value, stream, threshold, _lib.stream_addr()),
-                "pb_dropout",
-            )
-        return y
+
+def _launch_dropout(x, residual, seed, seed_value, stream, threshold):
+    x = x.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
+    y = torch.empty_like(x)
+    with _on_device_of(x):
+        _lib.check(
+            _lib.lib().pb_dropout(x.data_ptr(), _lib.addr(residual), y.data_ptr(), x.numel(), _lib.addr(seed),
+                                  seed_value, stream, threshold, _lib.stream_addr()),
+            "pb_dropout",
+        )
+    return y
 
 
 def dropout(x, p: float, seed: Union[int, torch.Tensor], residual: Optional[torch.Tensor] = None, stream: int = 0):

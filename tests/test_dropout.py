@@ -133,6 +133,15 @@ def test_kernel_seed_on_the_device():
 
 
 @gpu
+def test_kernel_second_derivative():
+    x = torch.randn(64, 40, device="cuda").bfloat16().requires_grad_(True)
+    g = torch.randn(64, 40, device="cuda").bfloat16().requires_grad_(True)
+    (dx,) = torch.autograd.grad(pf.dropout(x, 0.5, 3), x, g, create_graph=True)
+    (dg,) = torch.autograd.grad(dx, g, torch.ones_like(dx))
+    assert torch.equal(dg, pf.dropout(torch.ones_like(x), 0.5, 3))
+
+
+@gpu
 def test_kernel_beyond_32_bits():
     """Element numbers beyond 2^32 reach the counter's second word."""
     n = 2 ** 32 + 4099

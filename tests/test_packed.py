@@ -155,8 +155,8 @@ def test_refusals():
 
 # ------------------------------------------------------------------------------------------------ GPU
 def _read_tiles(layout, rows):
-    n = int(layout.counts[rows][0])
-    return layout.tiles[rows][: 4 * n].view(n, 4).tolist()
+    tiles, counts = layout.tiles(rows)
+    return tiles[: int(counts[0])].tolist()
 
 
 @gpu
@@ -181,11 +181,11 @@ def test_layout_kernel(case, errors):
                 want |= {(at, n, t, int(i == len(row))) for t in range(-(-n // rows))}
                 at += n
         got = _read_tiles(layout, rows)
-        assert len(got) == len(want) <= layout.max_tiles[rows] and {tuple(t) for t in got} == want
+        assert len(got) == len(want) <= len(layout.tiles(rows)[0]) and {tuple(t) for t in got} == want
         ranks = [t[2] if not t[3] else -1 for t in got]  # longest first, as far as there are buckets; padding last
         assert all(a >= b or min(a, b) >= 2047 for a, b in zip(ranks, ranks[1:]) if b >= 0) and sorted(ranks, key=lambda t: t == -1) == ranks
         half = [rows == 256 and t[1] <= 128 and not t[3] for t in got]  # the last ones before the padding
-        n_first, n_docs = layout.counts[rows][1:3].tolist()
+        n_first, n_docs = layout.tiles(rows)[1][1:3].tolist()
         assert n_docs == sum(1 for t in got if not t[3]) and half == [n_first <= i < n_docs for i in range(len(got))]
 
 
