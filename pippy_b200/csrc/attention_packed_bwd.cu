@@ -23,131 +23,9 @@
 //
 // P and dS are rounded to bf16, the type of their products' other operand; scores, accumulators, lse and delta are fp32.
 // The rotation of q and k is undone on dQ and dK in the epilogues, before their one rounding.
-#include "attention_packed.cuh"
+#include "attention_packed_bwd.cuh"
 
 namespace pbv {
-
-struct BwdArgs {
-  const __nv_bfloat16* o;  // pass 1: delta
-  long long o_stride;
-  const float* lse;  // [Hq, T] natural log
-  float* delta;      // [Hq, T]: written by pass 1, read by pass 2
-  __nv_bfloat16* out_a;  // pass 1: dQ; pass 2: dK
-  __nv_bfloat16* out_b;  // pass 2: dV
-  long long out_stride;
-  const float *cs, *sn;  // [table_rows, D / 2], null: no rotation
-  int table_rows;
-  long long T;
-  const Tile* tiles;  // of 128 rows
-  const int* count;
-  int max_tiles, Hq, Hkv;
-  float scale, scale_log2;
-  int causal;
-  int head_group;
-  int* err;
-};
-
-// kPolyPairs of 8 pairs of exponentials are computed on the FMA pipe (poly_exp2)
-constexpr int kPolyPairs = 4;
-
-__device__ __forceinline__ f32x2 exp2_pair(f32x2 x, bool poly) {
-  if (poly) return poly_exp2(x);
-  const float2 v = both(x);
-  return pair(fast_exp2(v.x), fast_exp2(v.y));
-}
-
-// Mask of a packed pair of bf16 of which the first `n` values stay (all for n >= 2, none for n <= 0).
-__device__ __forceinline__ uint32_t keep_below(int n) {
-  uint32_t m;
-  asm("shr.u32 %0, 0xffffffff, %1;" : "=r"(m) : "r"(max(32 - 16 * n, 0)));  // shifts by 32 and more give 0
-  return m;
-}
-
-// A warp's share of the rotation tables for 32 rows: columns [sub * D / 4, + D / 4) of each, on its way from memory while the
-// products that it is for are still running.  pos: position of the first row, < 0 for no rotation; rows: how many of the 32 are
-// the document's.
-template <int D>
-struct Turn {
-  static constexpr int kChunks = D / 64;  // of 16 columns
-  float4 cs[kChunks][4], sn[kChunks][4];
-  __device__ __forceinline__ void fetch(const BwdArgs& p, int pos, int rows, int sub, int lane) {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int r = u * 8 + (lane >> 2);
-        const bool in = pos >= 0 && r < rows && pos + r < p.table_rows;
-        const long long at = (long long)(pos + r) * (D / 2) + sub * (D / 4) + c * 16 + (lane & 3) * 4;
-        cs[c][u] = in ? __ldg(reinterpret_cast<const float4*>(p.cs + at)) : make_float4(1.f, 1.f, 1.f, 1.f);
-        sn[c][u] = in ? __ldg(reinterpret_cast<const float4*>(p.sn + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-  }
-};
-
-// 32 rows of an accumulator [128, D] to bf16, by one warp, a row per lane.  The warp's columns are [sub * D / 4, + D / 4) of each
-// half, so that a thread holds both elements of every pair that the rotation mixes.  A lane that read and wrote its
-// own row in global memory touched 32 lines with every access: 6 000 to 9 000 cycles for a tile of 128 x 128, several times
-// what its products take.  So the tables come, and the results leave, through `stage` (32 * D bytes of the warp's own), as
-// segments of 64 bytes.
-template <int D, bool kTurn>
-__device__ __forceinline__ void write_rows(uint32_t acc, int sub, float scale, const Turn<D>& turn, int rows, uint8_t* stage,
-                                           int lane, __nv_bfloat16* dst, long long stride) {
-  constexpr int N = D / 4;
-  constexpr int kPieces = D / 16;  // 16-byte pieces of a row's results
-  uint32_t out[N];                 // [half][N / 2]
-  // 64-byte rows: two of them share 128 bytes, hence the shift
-  auto at64 = [&](int row, int piece) { return reinterpret_cast<float4*>(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)); };
-#pragma unroll
-  for (int c = 0; c < N / 16; ++c) {
-    uint32_t a[16], b[16];
-    tmem_ld_32x16(acc + sub * N + c * 16, a);
-    tmem_ld_32x16(acc + D / 2 + sub * N + c * 16, b);
-    float4 cs[4], sn[4];
-    if (kTurn) {
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) *at64(u * 8 + (lane >> 2), lane & 3) = which == 0 ? turn.cs[c][u] : turn.sn[c][u];
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < 4; ++u) (which == 0 ? cs[u] : sn[u]) = *at64(lane, u);
-        __syncwarp();
-      }
-    }
-    tmem_ld_wait();
-    const f32x2 scale2 = pair(scale, scale);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      f32x2 f = mul2(pair(__uint_as_float(a[u * 2]), __uint_as_float(a[u * 2 + 1])), scale2);
-      f32x2 g = mul2(pair(__uint_as_float(b[u * 2]), __uint_as_float(b[u * 2 + 1])), scale2);
-      if (kTurn) {
-        const f32x2 cc = (u & 1) ? pair(cs[u >> 1].z, cs[u >> 1].w) : pair(cs[u >> 1].x, cs[u >> 1].y);
-        const f32x2 ss = (u & 1) ? pair(sn[u >> 1].z, sn[u >> 1].w) : pair(sn[u >> 1].x, sn[u >> 1].y);
-        const f32x2 x = fma2(g, ss, mul2(f, cc));
-        g = fma2(mul2(f, pair(-1.f, -1.f)), ss, mul2(g, cc));
-        f = x;
-      }
-      const float2 x = both(f), y = both(g);
-      out[c * 8 + u] = pack_bf16(x.x, x.y);
-      out[N / 2 + c * 8 + u] = pack_bf16(y.x, y.y);
-    }
-  }
-  auto at = [&](int row, int piece) {
-    const int x = kPieces == 8 ? (row & 7) : ((row >> 1) & 3);
-    return reinterpret_cast<uint4*>(stage + row * (kPieces * 16) + ((piece ^ x) << 4));
-  };
-#pragma unroll
-  for (int u = 0; u < kPieces; ++u) *at(lane, u) = make_uint4(out[u * 4], out[u * 4 + 1], out[u * 4 + 2], out[u * 4 + 3]);
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int r = i * (32 / kPieces) + lane / kPieces, u = lane % kPieces;
-    const uint4 w = *at(r, u);
-    const int col = (u < kPieces / 2 ? 0 : D / 2) + sub * N + (u % (kPieces / 2)) * 8;
-    if (r < rows) *reinterpret_cast<uint4*>(dst + r * stride + col) = w;
-  }
-  __syncwarp();
-}
 
 // ------------------------------------------------------------------------------------------------ pass 1: dQ
 constexpr int kStagesK = 3, kStagesV = 2;  // a K tile is read by S and, two products later, by dQ
@@ -155,16 +33,16 @@ constexpr int kDqThreads = 512;
 
 // Warps: 0 loads (TMA), 1 issues MMAs and owns TMEM, 2 clears what reaches beyond a document, 4..11 softmax (two per TMEM lane
 // quarter, 64 of a block's columns each), 12..15 bring an item's Q and dO from shared memory to TMEM and form delta.
-template <int D>
+template <int D, bool kTurn>
 __global__ void __launch_bounds__(kDqThreads, 1)
 packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                  const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, BwdArgs p) {
   constexpr int NCH = D / 64;
   constexpr int TILE_BYTES = NCH * kChunkBytes;
 
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  if (smem != smem_raw) {
+  // addresses of shared memory are constants, as long as nothing is computed from where it begins
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {  // the launch reserves no slack for re-alignment
     if (threadIdx.x == 0) atomicExch(p.err, ERR_BAD_ARG);
     return;
   }
@@ -189,15 +67,16 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_ready = s_full + 3;
   uint64_t* acc_full = s_full + 4;
+  uint8_t* sStage = reinterpret_cast<uint8_t*>(bars) + 256 + ItemRing::kBytes;  // D = 64 only
   ItemRing ring(reinterpret_cast<uint8_t*>(bars) + 256, s_full + 5);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5 + ItemRing::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int count = *p.count;
+  const int count = p.counts[1];  // longer documents only: see attention_packed_short.cu
   const int G = p.Hq / p.Hkv;
-  // an item: a tile of queries of head h and the blocks of keys that it sees (0: padding)
+  // an item: a tile of queries of head h and the blocks of keys that it sees
   Items items(count * p.Hq);
   bool ok = true;
   Tile tile;
@@ -209,7 +88,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
       tile = p.tiles[order.tile_rank];
       h = order.index;
-      nblk = tile.pad ? 0 : ((p.causal ? min(tile.len, tile.rank * 128 + 128) : tile.len) + 127) / 128;
+      nblk = ((p.causal ? min(tile.len, tile.rank * 128 + 128) : tile.len) + 127) / 128;
     }
     ok = ring.put(make_int4(tile.start, tile.len, tile.rank, h), make_int4(nblk, 0, 0, 0), make_int4(0, 0, 0, 0), lane, abort_flag);
     return ok && tile.start >= 0;
@@ -255,14 +134,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t tDP = tmem_base + 256;   // 128 columns; dS over them
   const uint32_t tAcc = tmem_base + 384;  // D columns
 
-  int it = 0;  // items with work so far
+  int it = 0;  // items so far
   int n = 0;   // blocks so far
   // launched with 128 registers a thread: 64 + 2 x 168 + 112 = 4 x 128
   if (warp < 4) {
     give_registers<64>();
     if (warp == 0) {
     while (ok && publish_next()) {
-      if (nblk == 0) continue;
       const int hkv = h / G;
       if (!(ok = warp_wait(stage_empty, (it & 1) ^ 1, abort_flag))) break;
       if (lane == 0) {
@@ -307,7 +185,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       __syncwarp();
     };
     while (ok && next_item()) {
-      if (nblk == 0) continue;
       if (!(ok = wait(res_ready, it & 1) && wait(&k_full[n % kStagesK], (n / kStagesK) & 1))) break;
       issue_scores(tS, tQ, sK + (n % kStagesK) * TILE_BYTES, s_full, nullptr);
       if (!(ok = wait(&v_full[n % kStagesV], (n / kStagesV) & 1))) break;
@@ -339,7 +216,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the k_raw barriers
     while (ok && next_item()) {
-      if (nblk == 0) continue;
       n += nblk;
       const int valid = tile.len - (nblk - 1) * 128;  // only an item's last block can reach beyond its document
       if (valid >= 128) continue;
@@ -355,7 +231,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     while (ok && next_item()) {
-      if (nblk == 0) continue;
       const bool row_ok = tile.rank * 128 + r < tile.len;
       const long long row = (long long)tile.start + tile.rank * 128 + r;
       const float lse2 = row_ok ? p.lse[(long long)h * p.T + row] * kLog2e : 0.f;
@@ -369,35 +244,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                    ? __ldg(reinterpret_cast<const uint4*>(p.o + ((long long)tile.start + tile.rank * 128 + first + k * kRows) * p.o_stride + h * D) + u)
                    : make_uint4(0, 0, 0, 0);
       if (!(ok = warp_wait(stage_full, it & 1, abort_flag))) break;
-      // 16-byte piece u of a row's 128 bytes lies at u ^ (row & 7)
-      auto piece = [&](const uint8_t* tile_s, int row_t, int u) {
-        return *reinterpret_cast<const uint4*>(tile_s + (u >> 3) * kChunkBytes + row_t * 128 + (((u & 7) ^ (row_t & 7)) << 4));
-      };
-      float dot[kLanes];
-#pragma unroll
-      for (int k = 0; k < kLanes; ++k) {
-        const uint4 x = piece(sDO, first + k * kRows, u);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
-        f32x2 sum = pair(0.f, 0.f);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)  // a bf16 is the upper half of its fp32
-          sum = fma2(pair(__uint_as_float(xs[e] << 16), __uint_as_float(xs[e] & 0xffff0000u)),
-                     pair(__uint_as_float(ys[e] << 16), __uint_as_float(ys[e] & 0xffff0000u)), sum);
-        const float2 v = both(sum);
-        dot[k] = v.x + v.y;
-      }
-      // the kLanes sums of every lane, added over the lanes of a row: each step halves the sums that a lane still carries, and
-      // lane u ends with row u of its half warp's
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) {
-        const bool upper = u & o;
-#pragma unroll
-        for (int k = 0; k < o; ++k) {
-          const float keep = upper ? dot[k + o] : dot[k], give = upper ? dot[k] : dot[k + o];
-          dot[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-        }
-      }
-      s_delta[first + u * kRows] = dot[0];
+      row_dots<D>(sDO, y, first, u, s_delta);
       __syncwarp();
       const float delta = s_delta[r];
       __syncwarp();
@@ -414,7 +261,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           uint32_t w[32];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const uint4 x = piece(which == 0 ? sQ : sDO, r, c * 8 + u);
+            const uint4 x = piece_of(which == 0 ? sQ : sDO, r, c * 8 + u);
             w[u * 4] = x.x, w[u * 4 + 1] = x.y, w[u * 4 + 2] = x.z, w[u * 4 + 3] = x.w;
           }
           tmem_st_32x32((which == 0 ? tQ : tDO) + lane_off + c * 32, w);
@@ -437,10 +284,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t my_s = tS + lane_off + sub * 64, my_dp = tDP + lane_off + sub * 64;
     while (ok && next_item()) {
       const int q0 = tile.rank * 128, q_idx = q0 + r;
-      if (nblk == 0) {
-        clear_rows<D>(p.out_a, p.out_stride, (long long)tile.start + q0, min(128, tile.len - q0), h * D, threadIdx.x - 128, 256);
-        continue;
-      }
       if (!(ok = warp_wait(res_ready, it & 1, abort_flag))) break;
       const float lse2 = s_stat[(it & 1) * 256 + r], delta = s_stat[(it & 1) * 256 + 128 + r];
       __syncwarp();
@@ -463,29 +306,25 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             (e & 7) < kPolyPairs);
         if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        tmem_ld_32x32(my_dp, t[0]);
-        tmem_ld_32x32(my_dp + 32, t[1]);
-        tmem_ld_wait();
         // dP was the only reader of this V tile; the last one's memory serves the epilogue first
         if (lane == 0 && j + 1 < nblk) mbar_arrive(&v_empty[n % kStagesV]);
         // the diagonal block (causal) and the one in which the document ends are masked, in the packed result: what a masked
         // score gave, Inf or NaN, is gone with it
         const int limit = j < nblk - 1 ? 64 : (p.causal ? min(tile.len, q_idx + 1) : tile.len) - j * 128 - sub * 64;
         const bool masked = j == nblk - 1;
+        by_chunks(my_dp, [&](int c, const uint32_t(&x)[16]) {
+          uint32_t pk[8];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 d = both(mul2(pr[c * 16 + e], add2(pair(__uint_as_float(t[c][2 * e]), __uint_as_float(t[c][2 * e + 1])), minus_delta)));
+          for (int e = 0; e < 8; ++e) {
+            const float2 d = both(mul2(pr[c * 8 + e], add2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), minus_delta)));
             pk[e] = pack_bf16(d.x, d.y);
           }
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] &= keep_below(limit - 2 * (c * 16 + e));
+            for (int e = 0; e < 8; ++e) pk[e] &= keep_below(limit - 2 * (c * 8 + e));
           }
-          tmem_st_32x16(my_dp + c * 16, pk);
-        }
+          tmem_st_32x8(my_dp + c * 8, pk);
+        });
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
@@ -494,14 +333,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!ok) break;
       const int first = q0 + quarter * 32;
       const int sv = (n - 1) % kStagesV;
-      Turn<D> turn;
-      if (p.cs) turn.fetch(p, first, tile.len - first, sub, lane);
+      Turn<D> turn(p, first, tile.len - first, sub, lane);
+      if (kTurn) turn.fetch(0);
       if (!(ok = warp_wait(acc_full, it & 1, abort_flag))) break;
       tc_fence_after_sync();
-      uint8_t* stage = sV + sv * TILE_BYTES + (warp - 4) * (32 * D);
+      uint8_t* stage = (D == 128 ? sV + sv * TILE_BYTES : sStage) + (warp - 4) * kStageBytes;
       __nv_bfloat16* dst = p.out_a + ((long long)tile.start + first) * p.out_stride + h * D;
-      if (p.cs) write_rows<D, true>(tAcc + lane_off, sub, p.scale, turn, tile.len - first, stage, lane, dst, p.out_stride);
-      else write_rows<D, false>(tAcc + lane_off, sub, p.scale, turn, tile.len - first, stage, lane, dst, p.out_stride);
+      write_rows<D, kTurn>(tAcc + lane_off, sub, p.scale, turn, tile.len - first, stage, lane, dst, p.out_stride);
       tc_fence_before_sync();
       fence_proxy_async_smem();  // the tile's next content comes by TMA
       __syncwarp();
@@ -519,16 +357,16 @@ constexpr int kDkvThreads = 384;
 
 // Warps: 0 loads (TMA), 1 issues MMAs and owns TMEM, 2 brings lse and delta of a block's queries, 3 clears what reaches beyond
 // a document, 4..11 softmax (two per TMEM lane quarter, 64 of a block's columns each).
-template <int D>
+template <int D, bool kTurn>
 __global__ void __launch_bounds__(kDkvThreads, 1)
 packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                   const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, BwdArgs p) {
   constexpr int NCH = D / 64;
   constexpr int TILE_BYTES = NCH * kChunkBytes;
 
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  if (smem != smem_raw) {
+  // addresses of shared memory are constants, as long as nothing is computed from where it begins
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {  // the launch reserves no slack for re-alignment
     if (threadIdx.x == 0) atomicExch(p.err, ERR_BAD_ARG);
     return;
   }
@@ -555,43 +393,45 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_ready = s_full + 3;
   uint64_t* acc_full = s_full + 4;
+  uint8_t* sStage = reinterpret_cast<uint8_t*>(bars) + 320 + ItemRing::kBytes;  // D = 64 only
   ItemRing ring(reinterpret_cast<uint8_t*>(bars) + 320, s_full + 5);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5 + ItemRing::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int count = *p.count;
-  const int G = p.Hq / p.Hkv;
+  const int count = p.counts[1];  // longer documents only: see attention_packed_short.cu
+  const int G = p.Hq / p.Hkv / p.split;  // query heads of an item
   // an item: rows [k0, k0 + 128) of a document as keys, blocks [first, tiles) of queries of G heads.  The table lists tiles by
   // the keys that queries see; the first keys are seen by the most queries.
   struct Item {
-    int start, len, hkv, kv_tile, first, tiles, blocks;
+    int start, len, hkv, part, kv_tile, first, tiles, blocks;
   };
-  Items items(count * p.Hkv);
+  Items items(count * p.Hkv * p.split);
   bool ok = true;
   Item w;
   auto decode = [&](int i) {
-    const TileOrder order = tile_order(i, count, p.Hkv, p.head_group);
+    const TileOrder order = tile_order(i, count, p.Hkv * p.split, p.head_group);
     const Tile tile = p.tiles[order.tile_rank];
-    w.start = tile.start, w.len = tile.len, w.hkv = order.index;
+    w.start = tile.start, w.len = tile.len, w.hkv = order.index / p.split;
+    w.part = order.index - w.hkv * p.split;
     w.tiles = (tile.len + 127) / 128;
     w.kv_tile = w.tiles - 1 - tile.rank;
     w.first = p.causal ? w.kv_tile : 0;
-    w.blocks = tile.pad ? 0 : G * (w.tiles - w.first);
+    w.blocks = G * (w.tiles - w.first);
   };
   auto publish_next = [&]() {  // by the loading warp; false after the last
     const int i = items.next();
     w.start = -1;
     if (i >= 0) decode(i);
-    ok = ring.put(make_int4(w.start, w.len, w.hkv, w.kv_tile), make_int4(w.first, w.tiles, w.blocks, 0), make_int4(0, 0, 0, 0), lane, abort_flag);
+    ok = ring.put(make_int4(w.start, w.len, w.hkv, w.kv_tile), make_int4(w.first, w.tiles, w.blocks, w.part), make_int4(0, 0, 0, 0), lane, abort_flag);
     return ok && w.start >= 0;
   };
   auto next_item = [&]() {  // by the others
     int4 a, b, c;
     if (!(ok = ring.get(a, b, c, lane, abort_flag))) return false;
     w.start = a.x, w.len = a.y, w.hkv = a.z, w.kv_tile = a.w;
-    w.first = b.x, w.tiles = b.y, w.blocks = b.z;
+    w.first = b.x, w.tiles = b.y, w.blocks = b.z, w.part = b.w;
     return w.start >= 0;
   };
 
@@ -633,18 +473,17 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t tDV = tmem_base + 256;   // D columns
   const uint32_t tDK = tmem_base + 384;   // D columns
 
-  int it = 0;  // items with work so far
+  int it = 0;  // items so far
   int n = 0;   // blocks so far
   // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
   if (warp < 4) {
     give_registers<72>();
     if (warp == 0) {
     while (ok && publish_next()) {
-      if (w.blocks == 0) continue;
       // rows beyond the document stay in their own accumulator rows, which are not written
       if (!(ok = warp_wait(k_empty, (it & 1) ^ 1, abort_flag))) break;
       if (lane == 0) load_tile<NCH>(sK, &tmK, k_full, w.hkv * D, w.start + w.kv_tile * 128);
-      int head = w.hkv * G, blk = w.first;
+      int head = (w.hkv * p.split + w.part) * G, blk = w.first;
       for (int b = 0; b < w.blocks; ++b, ++n) {
         const int sq = n % kStagesQ, sd = n % kStagesDO;
         const bool tail = w.len - blk * 128 < 128;
@@ -696,7 +535,6 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     };
     while (ok && next_item()) {
       const int blocks = w.blocks;
-      if (blocks == 0) continue;
       if (!(ok = wait(k_full, it & 1) && wait(&q_full[n % kStagesQ], (n / kStagesQ) & 1))) break;
       issue_scores(tS, sK, sQ + (n % kStagesQ) * TILE_BYTES, s_full, blocks == 1 ? k_empty : nullptr);
       if (!(ok = wait(v_full, it & 1) && wait(&do_full[n % kStagesDO], (n / kStagesDO) & 1))) break;
@@ -733,8 +571,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     };
     while (ok && next_item()) {
-      if (w.blocks == 0) continue;
-      int head = w.hkv * G, blk = w.first;
+      int head = (w.hkv * p.split + w.part) * G, blk = w.first;
       fetch(w, head, blk);
       for (int b = 0; b < w.blocks; ++b, ++n) {
         const int st = n % kStagesStat;
@@ -753,7 +590,6 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   } else {
     uint32_t q_phases = 0, do_phases = 0;  // of the raw barriers
     while (ok && next_item()) {
-      if (w.blocks == 0) continue;
       const int per_head = w.tiles - w.first, valid = w.len - (w.tiles - 1) * 128;
       if (valid >= 128) {
         n += w.blocks;
@@ -781,12 +617,6 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2);
     while (ok && next_item()) {
       const int k0 = w.kv_tile * 128;
-      if (w.blocks == 0) {
-        const int rows = min(128, w.len - k0);
-        clear_rows<D>(p.out_a, p.out_stride, (long long)w.start + k0, rows, w.hkv * D, threadIdx.x - 128, 256);
-        clear_rows<D>(p.out_b, p.out_stride, (long long)w.start + k0, rows, w.hkv * D, threadIdx.x - 128, 256);
-        continue;
-      }
       int blk = w.first;
       for (int b = 0; b < w.blocks; ++b, ++n) {
         const int st = n % kStagesStat;
@@ -832,38 +662,27 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
-        f32x2 dl[16];
+        f32x2 dl[32];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
+        for (int e = 0; e < 32; e += 2) {
           const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(minus_delta + e);
           dl[e] = d.x, dl[e + 1] = d.y;
         }
         if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        tmem_ld_32x32(my_dp, t[0]);
-        tmem_ld_32x32(my_dp + 32, t[1]);
-        tmem_ld_wait();
+        by_chunks(my_dp, [&](int c, const uint32_t(&x)[16]) {
+          uint32_t pk[8];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 v = both(mul2(pr[c * 16 + e], add2(pair(__uint_as_float(t[c][2 * e]), __uint_as_float(t[c][2 * e + 1])), dl[e])));
+          for (int e = 0; e < 8; ++e) {
+            const float2 v = both(mul2(pr[c * 8 + e], add2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), dl[c * 8 + e])));
             pk[e] = pack_bf16(v.x, v.y);
           }
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] &= ~keep_below(first - 2 * (c * 16 + e));
+            for (int e = 0; e < 8; ++e) pk[e] &= ~keep_below(first - 2 * (c * 8 + e));
           }
-          tmem_st_32x16(my_dp + c * 16, pk);
-          if (c == 0) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(minus_delta + 16 + e);
-              dl[e] = d.x, dl[e + 1] = d.y;
-            }
-          }
-        }
+          tmem_st_32x8(my_dp + c * 8, pk);
+        });
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
@@ -875,15 +694,21 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       if (!ok) break;
       const int first = k0 + quarter * 32;
-      Turn<D> turn;
-      if (p.cs) turn.fetch(p, first, w.len - first, sub, lane);
+      Turn<D> turn(p, first, w.len - first, sub, lane);
+      if (kTurn && p.split == 1) turn.fetch(0);
       if (!(ok = warp_wait(acc_full, it & 1, abort_flag))) break;
       tc_fence_after_sync();
       const long long at = ((long long)w.start + first) * p.out_stride + w.hkv * D;
-      uint8_t* stage = sV + (warp - 4) * (32 * D);  // V has been read; its next tile is loaded after this
-      if (p.cs) write_rows<D, true>(tDK + lane_off, sub, p.scale, turn, w.len - first, stage, lane, p.out_a + at, p.out_stride);
-      else write_rows<D, false>(tDK + lane_off, sub, p.scale, turn, w.len - first, stage, lane, p.out_a + at, p.out_stride);
-      write_rows<D, false>(tDV + lane_off, sub, 1.f, turn, w.len - first, stage, lane, p.out_b + at, p.out_stride);
+      uint8_t* stage = (D == 128 ? sV : sStage) + (warp - 4) * kStageBytes;  // V has been read; its next tile is loaded after this
+      if (p.split > 1) {
+        const long long pitch = (long long)p.Hkv * D, size = p.T * pitch;
+        float* dk = p.partial + w.part * 2 * size + ((long long)w.start + first) * pitch + w.hkv * D;
+        write_partial<D>(tDK + lane_off, sub, w.len - first, stage, lane, dk, pitch);
+        write_partial<D>(tDV + lane_off, sub, w.len - first, stage, lane, dk + size, pitch);
+      } else {
+        write_rows<D, kTurn>(tDK + lane_off, sub, p.scale, turn, w.len - first, stage, lane, p.out_a + at, p.out_stride);
+        write_rows<D, false>(tDV + lane_off, sub, 1.f, turn, w.len - first, stage, lane, p.out_b + at, p.out_stride);
+      }
       tc_fence_before_sync();
       fence_proxy_async_smem();
       __syncwarp();
@@ -895,15 +720,68 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   leave(abort_flag, warp, tmem_base);
 }
 
+// Adds the parts of dK and dV up, in their order; scale and rotation as in write_rows, zeros in padding.  Bound by bandwidth.  A
+// thread has 4 columns of both halves of a row.
 template <int D>
+__global__ void __launch_bounds__(256) packed_dkv_sum_kernel(BwdArgs p, const int* __restrict__ positions) {
+  constexpr int kPer = D / 8;
+  const int width = p.Hkv * D, per_row = p.Hkv * kPer;
+  const long long size = p.T * width;
+  for (long long t = blockIdx.x * (long long)blockDim.y + threadIdx.y; t < p.T; t += (long long)gridDim.x * blockDim.y) {
+    const int pos = positions[t];
+    for (int i = threadIdx.x; i < per_row; i += blockDim.x) {
+      const int h = i / kPer, c = (i - h * kPer) * 4, col = h * D + c;
+      float4 sum[4];  // dK low, dK high, dV low, dV high
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (pos >= 0) {
+        for (int part = 0; part < p.split; ++part)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(p.partial + (part * 2 + k / 2) * size + t * width + col + (k & 1) * (D / 2));
+            sum[k].x += x.x, sum[k].y += x.y, sum[k].z += x.z, sum[k].w += x.w;
+          }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sum[k].x *= p.scale, sum[k].y *= p.scale, sum[k].z *= p.scale, sum[k].w *= p.scale;
+        if (p.cs && pos < p.table_rows) {
+          const float4 cc = __ldg(reinterpret_cast<const float4*>(p.cs + (long long)pos * (D / 2) + c));
+          const float4 ss = __ldg(reinterpret_cast<const float4*>(p.sn + (long long)pos * (D / 2) + c));
+          const float4 f = sum[0], g = sum[1];
+          sum[0] = make_float4(f.x * cc.x + g.x * ss.x, f.y * cc.y + g.y * ss.y, f.z * cc.z + g.z * ss.z, f.w * cc.w + g.w * ss.w);
+          sum[1] = make_float4(g.x * cc.x - f.x * ss.x, g.y * cc.y - f.y * ss.y, g.z * cc.z - f.z * ss.z, g.w * cc.w - f.w * ss.w);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        __nv_bfloat16* dst = (k < 2 ? p.out_a : p.out_b) + t * p.out_stride + col + (k & 1) * (D / 2);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(sum[k].x, sum[k].y), pack_bf16(sum[k].z, sum[k].w));
+      }
+    }
+  }
+}
+
+// Items that share the query heads of a key head in pass 2.  An item there is G query heads of a tile of keys, so with few
+// key heads there are few items, and the longest alone can take longer than the average SM: one row of 16 384
+// tokens with 8 query heads on 2 key heads took 637 us unsplit, 333 blocks of 128 x 128 in the longest item against 214 on
+// the average SM, and MEASURED us split in two.  The parts cost 16 bytes per split, token and column of K, so the split stops
+// at three items for each of 148 SMs.
+static int split_for(int max_tiles, int Hq, int Hkv) {
+  const int G = Hq / Hkv;
+  for (int s = 1; s < G; ++s)
+    if (G % s == 0 && (long long)max_tiles * Hkv * s >= 3 * 148) return s;
+  return G;
+}
+
+template <int D, bool kTurn>
 static int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-                      BwdArgs p, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv, cudaStream_t stream) {
+                      BwdArgs p, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv, const int* positions, cudaStream_t stream) {
   constexpr int TILE = (D / 64) * kChunkBytes;
-  constexpr int SMEM1 = (2 + kStagesK + kStagesV) * TILE + 2560 + 256 + ItemRing::kBytes;
-  constexpr int SMEM2 = (2 + kStagesQ + kStagesDO) * TILE + kStagesStat * 1024 + 320 + ItemRing::kBytes;
+  constexpr int STAGE = D == 128 ? 0 : 8 * kStageBytes;  // a V tile of D = 128 has room for it
+  constexpr int SMEM1 = (2 + kStagesK + kStagesV) * TILE + 2560 + 256 + ItemRing::kBytes + STAGE;
+  constexpr int SMEM2 = (2 + kStagesQ + kStagesDO) * TILE + kStagesStat * 1024 + 320 + ItemRing::kBytes + STAGE;
   static_assert(SMEM1 <= 232448 && SMEM2 <= 232448, "one block's shared memory");
-  constexpr auto pass1 = packed_dq_kernel<D>;
-  constexpr auto pass2 = packed_dkv_kernel<D>;
+  constexpr auto pass1 = packed_dq_kernel<D, kTurn>;
+  constexpr auto pass2 = packed_dkv_kernel<D, kTurn>;
   if (cudaError_t e = pb::allow_smem<pass1, SMEM1>(); e != cudaSuccess) return (int)e;
   if (cudaError_t e = pb::allow_smem<pass2, SMEM2>(); e != cudaSuccess) return (int)e;
   p.out_a = dq;
@@ -912,9 +790,16 @@ static int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   pb_count_launch(1);
   p.out_a = dk;
   p.out_b = dv;
-  p.head_group = attention_head_group(p.max_tiles, p.Hkv);
-  pass2<<<resident_blocks((long long)p.max_tiles * p.Hkv), kDkvThreads, SMEM2, stream>>>(tq, tdo, tk, tv, p);
+  p.head_group = attention_head_group(p.max_tiles, p.Hkv * p.split);
+  pass2<<<resident_blocks((long long)p.max_tiles * p.Hkv * p.split), kDkvThreads, SMEM2, stream>>>(tq, tdo, tk, tv, p);
   pb_count_launch(1);
+  if (int rc = launch_short_bwd<D, kTurn>(tq, tdo, tk, tv, p, dq, dk, dv, stream)) return rc;
+  if (p.split > 1) {
+    const int x = p.Hkv * D / 8 < 256 ? (p.Hkv * D / 8 + 31) / 32 * 32 : 256, y = 256 / x;
+    const long long blocks = (p.T + y - 1) / y;
+    packed_dkv_sum_kernel<D><<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), dim3(x, y), 0, stream>>>(p, positions);
+    pb_count_launch(1);
+  }
   return (int)cudaGetLastError();
 }
 
@@ -924,11 +809,17 @@ extern "C" {
 
 // Layouts as in pb_packed_attention_fwd; q and k rotated as the forward saw them.  dq/dk/dv: bf16 rows of dqkv_stride, every
 // row written (zeros in padding).  cs/sn [table_rows, D / 2] (null: none): dq and dk are turned back by the row's position.
-// delta: [Hq, T] fp32 scratch of this call.  tiles: the layout's table of 128-row tiles.
+// scratch: pb_packed_attention_bwd_scratch bytes, 16-byte aligned, of this call alone.  tiles / counts: the layout's table of
+// 128-row tiles; positions: the layout's.
+long long pb_packed_attention_bwd_scratch(long long T, int Hq, int Hkv, int D, int max_tiles) {
+  const int split = pbv::split_for(max_tiles, Hq, Hkv);
+  return (T * Hq * 4 + 15) / 16 * 16 + (split > 1 ? split * 2 * T * Hkv * D * 4 : 0);
+}
+
 int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o,
-                            const float* lse, float* delta, void* dq, void* dk, void* dv, const float* cs,
-                            const float* sn, int table_rows, const int* tiles, const int* count, int max_tiles,
-                            long long T, int Hq, int Hkv, int D, long long q_stride, long long k_stride,
+                            const float* lse, void* scratch, void* dq, void* dk, void* dv, const float* cs,
+                            const float* sn, int table_rows, const int* tiles, const int* counts, int max_tiles,
+                            const int* positions, long long T, int Hq, int Hkv, int D, long long q_stride, long long k_stride,
                             long long v_stride, long long o_stride, long long do_stride, long long dqkv_stride,
                             float softmax_scale, int causal, int* err_dev, void* stream_) {
   using namespace pbv;
@@ -936,7 +827,7 @@ int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const 
   if (Hq < 1 || Hkv < 1 || Hq % Hkv != 0) return -2;
   if ((q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (o_stride % 8) || (do_stride % 8) || (dqkv_stride % 8)) return -3;
   uintptr_t all = 0;
-  for (const void* x : {o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)cs, (const void*)sn})
+  for (const void* x : {o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)cs, (const void*)sn, (const void*)scratch})
     all |= reinterpret_cast<uintptr_t>(x);
   if (all & 15) return -3;
   if (T < 1 || T > 0x7fffffffLL || max_tiles < 1 || (long long)max_tiles * Hq > 0x7fffffffLL) return -4;
@@ -952,13 +843,15 @@ int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const 
   p.o = reinterpret_cast<const __nv_bfloat16*>(o);
   p.o_stride = o_stride;
   p.lse = lse;
-  p.delta = delta;
+  p.delta = reinterpret_cast<float*>(scratch);
+  p.split = split_for(max_tiles, Hq, Hkv);
+  p.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(scratch) + (T * Hq * 4 + 15) / 16 * 16);
   p.out_stride = dqkv_stride;
   p.cs = cs, p.sn = sn;
   p.table_rows = table_rows;
   p.T = T;
   p.tiles = reinterpret_cast<const Tile*>(tiles);
-  p.count = count;
+  p.counts = counts;
   p.max_tiles = max_tiles;
   p.Hq = Hq, p.Hkv = Hkv;
   p.scale = softmax_scale;
@@ -967,8 +860,8 @@ int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const 
   p.err = err_dev;
   auto b = [](void* x) { return reinterpret_cast<__nv_bfloat16*>(x); };
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  return D == 128 ? launch_bwd<128>(tq, tk, tv, tdo, p, b(dq), b(dk), b(dv), stream)
-                  : launch_bwd<64>(tq, tk, tv, tdo, p, b(dq), b(dk), b(dv), stream);
+  const auto launch = D == 128 ? (cs ? launch_bwd<128, true> : launch_bwd<128, false>) : (cs ? launch_bwd<64, true> : launch_bwd<64, false>);
+  return launch(tq, tk, tv, tdo, p, b(dq), b(dk), b(dv), positions, stream);
 }
 
 }  // extern "C"

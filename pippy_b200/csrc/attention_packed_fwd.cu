@@ -42,10 +42,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   constexpr int NCH = D / 64;
   constexpr int TILE_BYTES = NCH * kChunkBytes;
 
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  if (smem != smem_raw) {
-    // the launch reserves no slack for re-alignment; refuse to run rather than overrun shared memory
+  // addresses of shared memory are constants, as long as nothing is computed from where it begins
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {  // the launch reserves no slack for re-alignment
     if (threadIdx.x == 0) atomicExch(p.err, ERR_BAD_ARG);
     return;
   }

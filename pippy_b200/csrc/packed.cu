@@ -11,10 +11,12 @@ namespace pbk {
 
 // Tiles are listed longest first: tile `rank` of a document sees rank + 1 tiles of keys (as a tile of keys it is seen by as
 // many tiles of queries when counted from the document's end), and a long tile that starts last runs alone at the end.
-// Ranks above the last bucket share it; they are all long.  Behind rank 0 come, in the table of 256 rows, the documents that
-// fill no more than half a tile (the attention forward takes two heads of such a one at a time), and then the padding.
+// Ranks above the last bucket share it; they are all long.  Behind rank 0 come the documents of 128 tokens
+// or fewer (the attention forward takes two heads of such a one at a time, its backward has a kernel for them), and then
+// the padding.
 constexpr int kRanks = 2048;
 constexpr int kBuckets = kRanks + 1;  // the last one; padding's is kBuckets
+constexpr int kCounters = kBuckets + 1;
 constexpr int kPlanThreads = 1024;
 constexpr int kChunk = 4096;  // tokens a block writes positions for
 
@@ -65,55 +67,67 @@ __device__ void plan_tiles(const LayoutArgs& a, int* s_hist, int* s_part) {
   }
   if (bad) atomicExch(a.err, ERR_LAYOUT);
   __syncthreads();
+  // Both tables at once: count the tiles of every bucket, sum the counts up, place the tiles.  A thread has a document; the
+  // tiles of a long one are shared by its warp.
   const int nseg = a.rows * (a.docs + 1);
-  for (int table = 0; table < 2; ++table) {
-    const int tile_rows = 128 << table;
-    for (int i = tid; i <= kBuckets; i += blockDim.x) s_hist[i] = 0;  // bucket kBuckets: padding, last
+  for (int i = tid; i < 2 * kCounters; i += blockDim.x) s_hist[i] = 0;
+  __syncthreads();
+  for (int sweep = 0; sweep < 2; ++sweep) {
+    auto add = [&](int table, int start, int len, int r, bool pad) {
+      const bool half = len <= 128;
+      const int bucket = pad ? kBuckets : (half ? kRanks : kRanks - 1 - min(r, kRanks - 1));  // high ranks first
+      const int at = atomicAdd(&s_hist[table * kCounters + bucket], 1);
+      if (sweep == 1 && at < a.max_tiles[table]) a.tiles[table][at] = Tile{start, len, r, pad ? 1 : 0};
+    };
+    for (int i0 = warp * 32; i0 < nseg; i0 += blockDim.x) {
+      const int i = i0 + lane;
+      const int2 seg = i < nseg ? a.segments[i] : make_int2(0, 0);
+      const bool pad = i % (a.docs + 1) == a.docs, is_long = seg.y > 512;
+      if (!is_long) {
+        for (int r = 0; r * 128 < seg.y; ++r) add(0, seg.x, seg.y, r, pad);
+        for (int r = 0; r * 256 < seg.y; ++r) add(1, seg.x, seg.y, r, pad);
+      }
+      for (unsigned left = __ballot_sync(0xffffffffu, is_long); left; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        const int start = __shfl_sync(0xffffffffu, seg.x, from), len = __shfl_sync(0xffffffffu, seg.y, from);
+        const bool its_pad = (i0 + from) % (a.docs + 1) == a.docs;
+        for (int r = lane; (long long)r * 128 < len; r += 32) add(0, start, len, r, its_pad);
+        for (int r = lane; (long long)r * 256 < len; r += 32) add(1, start, len, r, its_pad);
+      }
+    }
     __syncthreads();
-    for (int sweep = 0; sweep < 2; ++sweep) {  // count, then place
-      for (int i = warp; i < nseg; i += warps) {
-        const int2 seg = a.segments[i];
-        const bool pad = i % (a.docs + 1) == a.docs;
-        const int n = (seg.y + tile_rows - 1) / tile_rows;
-        for (int r = lane; r < n; r += 32) {
-          const bool half = table == 1 && seg.y <= 128;
-          const int bucket = pad ? kBuckets : (half ? kRanks : kRanks - 1 - min(r, kRanks - 1));  // high ranks first
-          const int at = atomicAdd(&s_hist[bucket], 1);
-          if (sweep == 1 && at < a.max_tiles[table]) a.tiles[table][at] = Tile{seg.x, seg.y, r, pad ? 1 : 0};
+    if (sweep == 0) {  // counts -> first places: an exclusive sum for each table, by half of the warps, a run of counters a thread
+      const int table = warp / (warps / 2), mine = tid - table * (kPlanThreads / 2);
+      int* hist = s_hist + table * kCounters;
+      const int per = (kCounters + kPlanThreads / 2 - 1) / (kPlanThreads / 2);
+      int sum = 0;
+      for (int k = 0; k < per; ++k)
+        if (mine * per + k < kCounters) sum += hist[mine * per + k];
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int below = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += below;
+      }
+      if (lane == 31) s_part[warp] = upto;
+      __syncthreads();
+      int base = upto - sum;
+      for (int k = table * (warps / 2); k < warp; ++k) base += s_part[k];
+      for (int k = 0; k < per; ++k) {
+        const int i = mine * per + k;
+        if (i < kCounters) {
+          const int n = hist[i];
+          hist[i] = base;
+          base += n;
         }
+      }
+      if (mine == kPlanThreads / 2 - 1) a.counts[table * 4] = min(base, a.max_tiles[table]);
+      __syncthreads();
+      if (mine == 0) {
+        a.counts[table * 4 + 1] = min(hist[kRanks], a.max_tiles[table]);
+        a.counts[table * 4 + 2] = min(hist[kBuckets], a.max_tiles[table]);
       }
       __syncthreads();
-      if (sweep == 0) {  // counts -> first places: an exclusive sum over kBuckets + 1 values, a run of them per thread
-        const int per = (kBuckets + 1 + kPlanThreads - 1) / kPlanThreads;
-        int sum = 0;
-        for (int k = 0; k < per; ++k)
-          if (tid * per + k <= kBuckets) sum += s_hist[tid * per + k];
-        int upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int below = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += below;
-        }
-        if (lane == 31) s_part[warp] = upto;
-        __syncthreads();
-        int base = upto - sum;
-        for (int w = 0; w < warp; ++w) base += s_part[w];
-        for (int k = 0; k < per; ++k) {
-          const int i = tid * per + k;
-          if (i <= kBuckets) {
-            const int n = s_hist[i];
-            s_hist[i] = base;
-            base += n;
-          }
-        }
-        if (tid == kPlanThreads - 1) a.counts[table * 4] = min(base, a.max_tiles[table]);
-        __syncthreads();
-        if (tid == 0) {
-          a.counts[table * 4 + 1] = min(s_hist[kRanks], a.max_tiles[table]);
-          a.counts[table * 4 + 2] = min(s_hist[kBuckets], a.max_tiles[table]);
-        }
-        __syncthreads();
-      }
     }
   }
 }
@@ -121,7 +135,7 @@ __device__ void plan_tiles(const LayoutArgs& a, int* s_hist, int* s_part) {
 // Block 0 plans the tiles, the others write the positions of kChunk tokens of one row each.  One launch of a few us: the
 // lengths stay on the device, so that nothing waits for the host.
 __global__ void __launch_bounds__(kPlanThreads) layout_kernel(LayoutArgs a) {
-  __shared__ int s_hist[kBuckets + 1];
+  __shared__ int s_hist[2 * kCounters];
   __shared__ int s_part[kPlanThreads / 32];
   if (blockIdx.x == 0) {
     plan_tiles(a, s_hist, s_part);

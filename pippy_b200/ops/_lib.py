@@ -47,7 +47,8 @@ SIGNATURES = {
     "pb_norm_bwd_res": "p" * 11 + "ip" "iiii" "p",
     "pb_norm_bwd_scratch_floats": "ii",
     "pb_norm_fwd": "p" * 6 + "iifip",
-    "pb_packed_attention_bwd": "p" * 12 + "i" "ppi" "liii" "llllll" "fipp",
+    "pb_packed_attention_bwd": "p" * 12 + "i" "ppip" "liii" "llllll" "fipp",
+    "pb_packed_attention_bwd_scratch": "liiii",
     "pb_packed_attention_fwd": "p" * 7 + "i" "liii" "llll" "fipp",
     "pb_packed_layout": "piii" "ppp" "ipi" "ppp",
     "pb_packed_rope": "plpl" "ppp" "liii" "pp",
@@ -82,6 +83,7 @@ def lib() -> ctypes.CDLL:
         handle.pb_launch_count.restype = c_ll
         handle.pb_last_cuda_error.restype = ctypes.c_char_p
         handle.pb_embed_sorted_scratch.restype = c_ll
+        handle.pb_packed_attention_bwd_scratch.restype = c_ll
         for name, types in SIGNATURES.items():
             getattr(handle, name).argtypes = [_TYPES[t] for t in types]
         _LIB = handle

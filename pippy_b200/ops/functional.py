@@ -586,12 +586,16 @@ class _SortedEmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, wte, wpe, positions, S: int, scale: float):
         T, H = ids.numel(), wte.shape[1]
-        table, ptable = _aligned(wte.detach()), None if wpe is None else _aligned(wpe.detach())
+        table, ptable = wte, wpe
+        if wte.data_ptr() % 16 or not wte.is_contiguous():
+            table = _aligned(wte.detach())
+        if wpe is not None and (wpe.data_ptr() % 16 or not wpe.is_contiguous()):
+            ptable = _aligned(wpe.detach())
         out = torch.empty(T, H, device=wte.device, dtype=wte.dtype)
         with _on_device_of(wte):
             _lib.check(
-                _lib.lib().pb_embed_scaled_fwd(_lib.addr(ids), _lib.addr(table), _lib.addr(ptable),
-                                               _lib.addr(positions), _lib.addr(out), T, H, S, wte.shape[0],
+                _lib.lib().pb_embed_scaled_fwd(ids.data_ptr(), table.data_ptr(), _lib.addr(ptable),
+                                               _lib.addr(positions), out.data_ptr(), T, H, S, wte.shape[0],
                                                0 if wpe is None else wpe.shape[0], scale, _lib.err_addr(wte.device),
                                                _lib.stream_addr()),
                 "pb_embed_scaled_fwd",
@@ -600,18 +604,19 @@ class _SortedEmbeddingFn(torch.autograd.Function):
         wte._pb_direct_grad = True
         if wpe is not None:
             wpe._pb_direct_grad = True
-        ctx.params = (wte, wpe)  # not saved tensors: see _LinearFn.forward
-        ctx.cfg = (S, scale)
+        ctx.cfg = (wte, wpe, S, scale)  # parameters are not saved tensors: see _LinearFn.forward
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _no_second_derivative("embedding with sorted gradients")
         ids, positions = ctx.saved_tensors
-        wte, wpe = ctx.params
-        S, scale = ctx.cfg
-        d2 = _aligned(dout)
-        _run_or_defer(lambda: _embed_sorted_wgrad(ids, positions, d2, wte, wpe, S, scale))
+        dout = _aligned(dout)
+        if current_deferral() is None:
+            _embed_sorted_wgrad(ids, positions, dout, *ctx.cfg)
+        else:
+            cfg = ctx.cfg
+            _run_or_defer(lambda: _embed_sorted_wgrad(ids, positions, dout, *cfg))
         return None, None, None, None, None, None
 
 
@@ -624,16 +629,17 @@ def _embed_sorted_wgrad(ids, positions, dout, wte, wpe, S, scale):
         return mg is not None and mg.dtype == torch.float32 and mg.is_contiguous() and mg.data_ptr() % 16 == 0
 
     # the kernel adds to the parameters' fp32 buffers, or it writes gradients whole, in the parameters' type
-    direct = all(has_buffer(p) for p in params)
+    direct = all(map(has_buffer, params))
     grads = [p.main_grad if direct else torch.empty(p.shape, dtype=p.dtype, device=p.device) for p in params]
-    where = {id(p): _lib.addr(g) for p, g in zip(params, grads)}
+    gw = grads[0].data_ptr() if wte.requires_grad else None
+    gp = grads[-1].data_ptr() if wpe is not None and wpe.requires_grad else None
     lib = _lib.lib()
     scratch = torch.empty(lib.pb_embed_sorted_scratch(T, H, len(params)), dtype=torch.uint8, device=dout.device)
     with _on_device_of(dout):
         _lib.check(
-            lib.pb_embed_sorted_bwd(_lib.addr(ids), _lib.addr(positions), _lib.addr(dout), where.get(id(wte)),
-                                    where.get(id(wpe)), T, H, S, wte.shape[0], 0 if wpe is None else wpe.shape[0],
-                                    scale, int(not direct), _lib.addr(scratch), _lib.stream_addr()),
+            lib.pb_embed_sorted_bwd(ids.data_ptr(), _lib.addr(positions), dout.data_ptr(), gw, gp, T, H, S, wte.shape[0],
+                                    0 if wpe is None else wpe.shape[0], scale, int(not direct), scratch.data_ptr(),
+                                    _lib.stream_addr()),
             "pb_embed_sorted_bwd",
         )
         if not direct:
@@ -671,8 +677,11 @@ def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 
                 wpe.shape[1:] != wte.shape[1:] or wpe.dtype != wte.dtype or wpe.device != wte.device)):
             raise ValueError("tables: [rows, H] of one type on one device, H a multiple of 8")
         if positions is not None:
-            positions = positions.reshape(-1).to(torch.int32).contiguous()
-        return _SortedEmbeddingFn.apply(ids.reshape(-1).long().contiguous(), wte, wpe, positions, S, float(scale))
+            if positions.dtype != torch.int32 or not positions.is_contiguous():
+                positions = positions.to(torch.int32).contiguous()
+        if ids.dtype != torch.int64 or not ids.is_contiguous():
+            ids = ids.long().contiguous()
+        return _SortedEmbeddingFn.apply(ids, wte, wpe, positions, S, float(scale))
     if plain:
         out = F.embedding(ids.reshape(-1), wte)
         if wpe is not None:
@@ -811,14 +820,16 @@ class _PackedAttentionFn(torch.autograd.Function):
         with _on_device_of(qkv):
             do = _aligned(do)
             dqkv = torch.empty(T, nq + 2 * nk, device=qkv.device, dtype=qkv.dtype)
-            delta = torch.empty(Hq, T, device=qkv.device, dtype=torch.float32)
+            lib = _lib.lib()
+            scratch = torch.empty(lib.pb_packed_attention_bwd_scratch(T, Hq, Hkv, D, layout._most[0]), dtype=torch.uint8,
+                                  device=qkv.device)
             t128, _, counts, _ = layout._addresses()
             q, v, d, pitch = qk.data_ptr(), qkv.data_ptr() + 2 * (nq + nk), dqkv.data_ptr(), qk.stride(0)
             _lib.check(
-                _lib.lib().pb_packed_attention_bwd(
-                    do.data_ptr(), q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), delta.data_ptr(), d, d + 2 * nq,
+                lib.pb_packed_attention_bwd(
+                    do.data_ptr(), q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), scratch.data_ptr(), d, d + 2 * nq,
                     d + 2 * (nq + nk), _lib.addr(cos), _lib.addr(sin), 0 if cos is None else cos.shape[0], t128, counts,
-                    layout._most[0], T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, nq, nq + 2 * nk, scale, int(causal),
+                    layout._most[0], layout.positions.data_ptr(), T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, nq, nq + 2 * nk, scale, int(causal),
                     _lib.err_addr(qkv.device), _lib.stream_addr()),
                 "pb_packed_attention_bwd",
             )

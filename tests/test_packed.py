@@ -184,7 +184,7 @@ def test_layout_kernel(case, errors):
         assert len(got) == len(want) <= len(layout.tiles(rows)[0]) and {tuple(t) for t in got} == want
         ranks = [t[2] if not t[3] else -1 for t in got]  # longest first, as far as there are buckets; padding last
         assert all(a >= b or min(a, b) >= 2047 for a, b in zip(ranks, ranks[1:]) if b >= 0) and sorted(ranks, key=lambda t: t == -1) == ranks
-        half = [rows == 256 and t[1] <= 128 and not t[3] for t in got]  # the last ones before the padding
+        half = [t[1] <= 128 and not t[3] for t in got]  # the last ones before the padding
         n_first, n_docs = layout.tiles(rows)[1][1:3].tolist()
         assert n_docs == sum(1 for t in got if not t[3]) and half == [n_first <= i < n_docs for i in range(len(got))]
 
