@@ -244,7 +244,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                    ? __ldg(reinterpret_cast<const uint4*>(p.o + ((long long)tile.start + tile.rank * 128 + first + k * kRows) * p.o_stride + h * D) + u)
                    : make_uint4(0, 0, 0, 0);
       if (!(ok = warp_wait(stage_full, it & 1, abort_flag))) break;
-      row_dots<D>(sDO, y, first, u, s_delta);
+      row_dots<D, kLanes>(sDO, y, first, u, s_delta);
       __syncwarp();
       const float delta = s_delta[r];
       __syncwarp();
@@ -292,18 +292,20 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       for (int j = 0; j < nblk; ++j, ++n) {
         if (!(ok = warp_wait(s_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        uint32_t t[2][32];
         f32x2 pr[32];
-        tmem_ld_32x32(my_s, t[0]);
-        tmem_ld_32x32(my_s + 32, t[1]);
-        tmem_ld_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_read);
+        {
+          uint32_t t[2][32];
+          tmem_ld_32x32(my_s, t[0]);
+          tmem_ld_32x32(my_s + 32, t[1]);
+          tmem_ld_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_read);
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse),
-                            (e & 7) < kPolyPairs);
+          for (int e = 0; e < 32; ++e)
+            pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse),
+                              (e & 7) < kPolyPairs);
+        }
         if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
         // dP was the only reader of this V tile; the last one's memory serves the epilogue first
@@ -633,14 +635,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         if (!(ok = warp_wait(s_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        uint32_t t[2][32];
-        tmem_ld_32x32(my_s, t[0]);
-        tmem_ld_32x32(my_s + 32, t[1]);
-        tmem_ld_wait();
+        by_chunks(my_s, [&](int c, const uint32_t(&x)[16]) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, pr[e]),
-                            (e & 7) < kPolyPairs);
+          for (int e = 0; e < 8; ++e)
+            pr[c * 8 + e] = exp2_pair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, pr[c * 8 + e]), e < kPolyPairs);
+        });
         // queries before this key are masked, in the packed results
         const bool masked = p.causal && blk == w.kv_tile;
         const int first = r - sub * 64;

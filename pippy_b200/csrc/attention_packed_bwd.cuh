@@ -81,6 +81,32 @@ struct Turn {
   }
 };
 
+// A lane's D / 2 results, bf16 pairs [half][D / 8] of its row, to global memory through `stage`.
+template <int D>
+__device__ __forceinline__ void store_rows(const uint32_t (&out)[D / 4], int sub, int rows, uint8_t* stage, int lane,
+                                           __nv_bfloat16* dst, long long stride) {
+  constexpr int N = D / 4;
+  constexpr int kPieces = D / 16;          // 16-byte pieces of a row's results
+  constexpr int kRowsPer = 32 / kPieces;  // rows of one access
+  auto at = [&](int row, int piece) {
+    const int x = kPieces == 8 ? (row & 7) : ((row >> 1) & 3);
+    return reinterpret_cast<uint4*>(stage + row * (kPieces * 16) + ((piece ^ x) << 4));
+  };
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) *at(lane, u) = make_uint4(out[u * 4], out[u * 4 + 1], out[u * 4 + 2], out[u * 4 + 3]);
+  __syncwarp();
+  const int u = lane % kPieces;
+  dst += (lane / kPieces) * stride + (u < kPieces / 2 ? 0 : D / 2) + sub * N + (u % (kPieces / 2)) * 8;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int r = i * kRowsPer + lane / kPieces;
+    const uint4 w = *at(r, u);
+    if (r < rows) *reinterpret_cast<uint4*>(dst) = w;
+    dst += kRowsPer * stride;
+  }
+  __syncwarp();
+}
+
 // 32 rows of an accumulator [128, D] to bf16, by one warp, a row per lane.  The warp's columns are [sub * D / 4, + D / 4) of each
 // half, so that a thread holds both elements of every pair that the rotation mixes.  A lane that read and wrote its
 // own row in global memory touched 32 lines with every access: 6 000 to 9 000 cycles for a tile of 128 x 128, several times
@@ -90,8 +116,7 @@ template <int D, bool kTurn>
 __device__ __forceinline__ void write_rows(uint32_t acc, int sub, float scale, Turn<D>& turn, int rows, uint8_t* stage,
                                            int lane, __nv_bfloat16* dst, long long stride) {
   constexpr int N = D / 4;
-  constexpr int kPieces = D / 16;  // 16-byte pieces of a row's results
-  uint32_t out[N];                 // [half][N / 2]
+  uint32_t out[N];  // [half][N / 2]
   const f32x2 scale2 = pair(scale, scale);
   // 64-byte rows, cosines and then sines; two of them share 128 bytes, hence the shift
   const uint32_t put_at = (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
@@ -136,24 +161,7 @@ __device__ __forceinline__ void write_rows(uint32_t acc, int sub, float scale, T
     }
     __syncwarp();
   }
-  constexpr int kRowsPer = 32 / kPieces;  // rows of one access
-  auto at = [&](int row, int piece) {
-    const int x = kPieces == 8 ? (row & 7) : ((row >> 1) & 3);
-    return reinterpret_cast<uint4*>(stage + row * (kPieces * 16) + ((piece ^ x) << 4));
-  };
-#pragma unroll
-  for (int u = 0; u < kPieces; ++u) *at(lane, u) = make_uint4(out[u * 4], out[u * 4 + 1], out[u * 4 + 2], out[u * 4 + 3]);
-  __syncwarp();
-  const int u = lane % kPieces;
-  dst += (lane / kPieces) * stride + (u < kPieces / 2 ? 0 : D / 2) + sub * N + (u % (kPieces / 2)) * 8;
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int r = i * kRowsPer + lane / kPieces;
-    const uint4 w = *at(r, u);
-    if (r < rows) *reinterpret_cast<uint4*>(dst) = w;
-    dst += kRowsPer * stride;
-  }
-  __syncwarp();
+  store_rows<D>(out, sub, rows, stage, lane, dst, stride);
 }
 
 // The same rows in fp32, as they are: a part of dK or dV.  The warp's columns are [sub * D / 4, + D / 4) of each half here too.
@@ -180,19 +188,52 @@ __device__ __forceinline__ void write_partial(uint32_t acc, int sub, int rows, u
   }
 }
 
+// write_rows with the tables of the lane's row in registers, [pair of columns]: for documents that begin at the tile's first row
+// they are the same in every item.
+template <int D, bool kTurn>
+__device__ __forceinline__ void write_rows_held(uint32_t acc, int sub, float scale, const f32x2 (&cs)[D / 8], const f32x2 (&sn)[D / 8],
+                                                bool turn, int rows, uint8_t* stage, int lane, __nv_bfloat16* dst,
+                                                long long stride) {
+  constexpr int N = D / 4;
+  uint32_t out[N];
+  const f32x2 scale2 = pair(scale, scale);
+#pragma unroll
+  for (int c = 0; c < N / 16; ++c) {
+    uint32_t a[16], b[16];
+    tmem_ld_32x16(acc + sub * N + c * 16, a);
+    tmem_ld_32x16(acc + D / 2 + sub * N + c * 16, b);
+    tmem_ld_wait();
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      f32x2 f = mul2(pair(__uint_as_float(a[u * 2]), __uint_as_float(a[u * 2 + 1])), scale2);
+      f32x2 g = mul2(pair(__uint_as_float(b[u * 2]), __uint_as_float(b[u * 2 + 1])), scale2);
+      if (kTurn && turn) {
+        const f32x2 cc = cs[c * 8 + u], ss = sn[c * 8 + u];
+        const f32x2 x = fma2(g, ss, mul2(f, cc));
+        g = fma2(mul2(f, pair(-1.f, -1.f)), ss, mul2(g, cc));
+        f = x;
+      }
+      const float2 x = both(f), y = both(g);
+      out[c * 8 + u] = pack_bf16(x.x, x.y);
+      out[N / 2 + c * 8 + u] = pack_bf16(y.x, y.y);
+    }
+  }
+  store_rows<D>(out, sub, rows, stage, lane, dst, stride);
+}
+
 // 16-byte piece `u` of row `row` of a tile: inside the 128 bytes of a chunk it lies at u ^ (row & 7).
 __device__ __forceinline__ uint4 piece_of(const uint8_t* tile, int row, int u) {
   return *reinterpret_cast<const uint4*>(tile + (u >> 3) * kChunkBytes + row * 128 + (((u & 7) ^ (row & 7)) << 4));
 }
 
-// delta = dO O of a warp's 32 rows to out[row].  D / 8 lanes share a row, so that O is read in whole lines: lane has piece u of
-// rows first + k * 32 / (D / 8) in y[k], and dO comes from its tile.
-template <int D>
-__device__ __forceinline__ void row_dots(const uint8_t* tile_do, const uint4 (&y)[D / 8], int first, int u, float* out) {
+// delta = dO O of a warp's rows to out[row].  D / 8 lanes share a row, so that O is read in whole lines: lane has piece u of
+// rows first + k * 32 / (D / 8) in y[k], kCount of them, and dO comes from its tile.
+template <int D, int kCount>
+__device__ __forceinline__ void row_dots(const uint8_t* tile_do, const uint4 (&y)[kCount], int first, int u, float* out) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;
-  float dot[kLanes];
+  float dot[kCount];
 #pragma unroll
-  for (int k = 0; k < kLanes; ++k) {
+  for (int k = 0; k < kCount; ++k) {
     const uint4 x = piece_of(tile_do, first + k * kRows, u);
     const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
     f32x2 sum = pair(0.f, 0.f);
@@ -203,10 +244,14 @@ __device__ __forceinline__ void row_dots(const uint8_t* tile_do, const uint4 (&y
     const float2 v = both(sum);
     dot[k] = v.x + v.y;
   }
-  // the kLanes sums of every lane, added over the lanes of a row: each step halves the sums that a lane still carries, and
-  // lane u ends with row u of its group's
+  // the kCount sums of every lane, added over the lanes of a row: each step halves the sums that a lane still carries, and lane
+  // u ends with row u % kCount of its group's
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) {
+  for (int o = kLanes / 2; o >= kCount; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+#pragma unroll
+  for (int o = kCount / 2; o > 0; o >>= 1) {
     const bool upper = u & o;
 #pragma unroll
     for (int k = 0; k < o; ++k) {
@@ -214,7 +259,7 @@ __device__ __forceinline__ void row_dots(const uint8_t* tile_do, const uint4 (&y
       dot[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
     }
   }
-  out[first + u * kRows] = dot[0];
+  if (u < kCount) out[first + u * kRows] = dot[0];
 }
 
 // Documents of 128 tokens or fewer, and padding (attention_packed_short.cu).

@@ -8,16 +8,16 @@
 //     P, dS -> shared memory                 bf16 [query][key], which serves as three operands
 //     dV += P^T dO, dK += dS^T Q             P and dS read key-major
 //     dQ = dS K                              dS read query-major; over dP's columns in TMEM
-// The chain of one head is serial; what overlaps it are the next head's loads and its S, and the O rows for its delta.  The
+// The chain of one head is serial; what overlaps it are the next head's loads and its S.  The
 // products run over the document's tokens, rounded up to 16, and not over the tile.
 // Roundings as in the longer documents' kernels.
-// Warps: 0 loads (TMA), 1 issues MMAs and owns TMEM, 2 clears what reaches beyond the document, 4..11 softmax and
-// epilogue (two per TMEM lane quarter, 64 keys each), 12..15 form delta.
+// Warps: 0 loads (TMA), 1 issues MMAs and owns TMEM, 2 clears what reaches beyond the document, 4..11 softmax, delta and
+// epilogue (two per TMEM lane quarter, 64 keys each).
 #include "attention_packed_bwd.cuh"
 
 namespace pbv {
 
-constexpr int kShortThreads = 512;
+constexpr int kShortThreads = 384;
 
 template <int D, bool kTurn>
 __global__ void __launch_bounds__(kShortThreads, 1)
@@ -40,9 +40,8 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint8_t* sDO = sQ + 2 * TILE_BYTES;
   uint8_t* sP = sDO + TILE_BYTES;  // and, when its product is done, the epilogue's memory
   uint8_t* sDS = sP + PAIR_BYTES;
-  float* s_stat = reinterpret_cast<float*>(sDS + PAIR_BYTES);  // [step & 1][lse2, delta][128]
-  float* s_delta = s_stat + 512;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_delta + 128);
+  float* s_delta = reinterpret_cast<float*>(sDS + PAIR_BYTES);  // [step & 1][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_delta + 256);
   uint64_t* k_full = bars;
   uint64_t* k_raw = bars + 1;
   uint64_t* v_full = bars + 2;
@@ -53,16 +52,16 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint64_t* do_full = bars + 10;
   uint64_t* do_raw = bars + 11;
   uint64_t* do_empty = bars + 12;
-  uint64_t* stat_full = bars + 13;   // [2]
-  uint64_t* stat_empty = bars + 15;  // [2]
-  uint64_t* s_full = bars + 17;
-  uint64_t* p_ready = bars + 18;
-  uint64_t* dp_full = bars + 19;
-  uint64_t* ds_ready = bars + 20;
-  uint64_t* done = bars + 21;      // all products of a step
-  uint64_t* epi_done = bars + 22;  // its results have left TMEM and sP
-  ItemRing ring(reinterpret_cast<uint8_t*>(bars) + 320, bars + 23);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23 + ItemRing::kBars);
+  uint64_t* delta_ready = bars + 13;
+  uint64_t* s_full = bars + 14;
+  uint64_t* p_ready = bars + 15;
+  uint64_t* dp_full = bars + 16;
+  uint64_t* ds_ready = bars + 17;
+  uint64_t* done = bars + 18;      // all products of a step
+  uint64_t* epi_done = bars + 19;  // its results have left TMEM and sP
+  constexpr int kBars = 20;
+  ItemRing ring(reinterpret_cast<uint8_t*>(bars) + 320, bars + kBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars + ItemRing::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -95,16 +94,11 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 23; ++i) {
-      int arrivals = 1;
-      if (&bars[i] == do_empty) arrivals = 5;                                                    // products, delta
-      if (&bars[i] == stat_full || &bars[i] == stat_full + 1) arrivals = 4;                      // delta's warps
-      if (&bars[i] == stat_empty || &bars[i] == stat_empty + 1 || &bars[i] == p_ready || &bars[i] == ds_ready ||
-          &bars[i] == epi_done)
-        arrivals = 8;  // softmax
-      mbar_init(&bars[i], arrivals);
+    for (int i = 0; i < kBars; ++i) {
+      const uint64_t* bar = &bars[i];
+      mbar_init(&bars[i], bar == delta_ready || bar == p_ready || bar == ds_ready || bar == epi_done ? 8 : 1);  // 8: softmax
     }
-    ring.init(14);  // MMA, clearing, softmax, delta
+    ring.init(10);  // MMA, clearing, softmax
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -120,9 +114,9 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 
   int it = 0;  // documents so far
   int n = 0;   // steps (a query head of a document) so far
-  // launched with 128 registers a thread: 64 + 2 x 168 + 112 = 4 x 128
+  // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
   if (warp < 4) {
-    give_registers<64>();
+    give_registers<72>();
     if (warp == 0) {
       while (ok && publish_next()) {
         if (pad) continue;
@@ -222,36 +216,8 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           ok = clear(sQ + (n & 1) * TILE_BYTES, &q_raw[n & 1], 1 + (n & 1), &q_full[n & 1]) && clear(sDO, do_raw, 3, do_full);
       }
     }
-  } else if (warp >= 12) {
-    give_registers<112>();
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes to a row of O
-    const int u = lane % kLanes, first = quarter * 32 + lane / kLanes;
-    while (ok && next_item()) {
-      if (pad) continue;
-      for (int g = 0; g < G; ++g, ++n) {
-        const int h = (hkv * p.split + part) * G + g;
-        uint4 y[kLanes];
-#pragma unroll
-        for (int k = 0; k < kLanes; ++k)
-          y[k] = first + k * kRows < len ? __ldg(reinterpret_cast<const uint4*>(p.o + ((long long)start + first + k * kRows) * p.o_stride + h * D) + u)
-                                         : make_uint4(0, 0, 0, 0);
-        const float lse2 = r < len ? p.lse[(long long)h * p.T + start + r] * kLog2e : 0.f;
-        if (!(ok = warp_wait(do_full, n & 1, abort_flag) && warp_wait(&stat_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag))) break;
-        row_dots<D>(sDO, y, first, u, s_delta);
-        __syncwarp();
-        s_stat[(n & 1) * 256 + r] = lse2;
-        s_stat[(n & 1) * 256 + 128 + r] = r < len ? s_delta[r] : 0.f;
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&stat_full[n & 1]);
-          mbar_arrive(do_empty);
-        }
-      }
-    }
   } else {
-    take_registers<168>();
+    take_registers<216>();
     const int sub = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;  // query row of this thread, and its key row in the epilogue of dK and dV
@@ -259,9 +225,41 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     const uint32_t my_s = tS + lane_off + sub * 64, my_dp = tDP + lane_off + sub * 64;
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2);
     uint8_t* stage = sP + (warp - 4) * kStageBytes;
-    while (ok && next_item()) {
-      const int head0 = (hkv * p.split + part) * G;
-      if (pad) {
+    // the tables of row r: every document begins at row 0 of its tile
+    f32x2 cs[D / 8], sn[D / 8];
+    if (kTurn) {
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) {
+        float4 c = make_float4(1.f, 1.f, 1.f, 1.f), t = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < p.table_rows) {
+          c = __ldg(reinterpret_cast<const float4*>(p.cs + r * (D / 2) + sub * (D / 4)) + u);
+          t = __ldg(reinterpret_cast<const float4*>(p.sn + r * (D / 2) + sub * (D / 4)) + u);
+        }
+        cs[u * 2] = pair(c.x, c.y), cs[u * 2 + 1] = pair(c.z, c.w);
+        sn[u * 2] = pair(t.x, t.y), sn[u * 2 + 1] = pair(t.z, t.w);
+      }
+    }
+    // delta of 16 rows is this warp's: D / 8 lanes to a row
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kCount = 16 / kRows;
+    const int piece_u = lane % kLanes, dot_first = (warp - 4) * 16 + lane / kLanes;
+    // O and lse of a step are fetched under the epilogue of the step before, whose item may be another
+    uint4 y[kCount];
+    float lse2 = 0.f;
+    auto fetch = [&](int h) {
+#pragma unroll
+      for (int k = 0; k < kCount; ++k)
+        y[k] = dot_first + k * kRows < len
+                   ? __ldg(reinterpret_cast<const uint4*>(p.o + ((long long)start + dot_first + k * kRows) * p.o_stride + h * D) + piece_u)
+                   : make_uint4(0, 0, 0, 0);
+      lse2 = r < len ? p.lse[(long long)h * p.T + start + r] * kLog2e : 0.f;
+    };
+    auto next_document = [&]() {  // clears the padding that comes on the way
+      while (next_item()) {
+        const int head0 = (hkv * p.split + part) * G;
+        if (!pad) {
+          fetch(head0);
+          return true;
+        }
         const int first = rank * 128, rows = min(128, len - first);
         for (int g = 0; g < G; ++g)
           clear_rows<D>(dq, p.out_stride, (long long)start + first, rows, (head0 + g) * D, threadIdx.x - 128, 256);
@@ -269,32 +267,26 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           clear_rows<D>(dk, p.out_stride, (long long)start + first, rows, hkv * D, threadIdx.x - 128, 256);
           clear_rows<D>(dv, p.out_stride, (long long)start + first, rows, hkv * D, threadIdx.x - 128, 256);
         }
-        continue;
       }
+      return false;
+    };
+    bool more = next_document();
+    while (ok && more) {
+      const int head0 = (hkv * p.split + part) * G, hkv0 = hkv, part0 = part;
       const int n16 = (len + 15) & ~15;
-      const bool active = quarter * 32 < n16 && sub * 64 < n16;  // this warp has scores that a product reads
-      const int limit = r < len ? (p.causal ? min(len, r + 1) : len) - sub * 64 : 0;
+      // which of its scores a product reads, and which of these are not masked
+      const bool active = quarter * 32 < n16 && sub * 64 < n16;
+      const bool zeros = p.causal && sub * 64 > quarter * 32 + 31;
+      const bool row_ok = r < len;
+      const int limit = row_ok ? (p.causal ? min(len, r + 1) : len) - sub * 64 : 0;
+      const bool masked = __any_sync(0xffffffffu, limit < 64);
       const int first = quarter * 32, rows = len - first;
       const long long row = (long long)start + first;
       for (int g = 0; g < G; ++g, ++n) {
-        if (!(ok = warp_wait(&stat_full[n & 1], (n >> 1) & 1, abort_flag))) break;
-        const float lse2 = s_stat[(n & 1) * 256 + r], delta = s_stat[(n & 1) * 256 + 128 + r];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&stat_empty[n & 1]);
-        const f32x2 minus_lse = pair(-lse2, -lse2), minus_delta = pair(-delta, -delta);
+        const int h = head0 + g;
+        const f32x2 minus_lse = pair(-lse2, -lse2);
         if (!(ok = warp_wait(s_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        f32x2 pr[32];
-        if (active) {
-          uint32_t t[2][32];
-          tmem_ld_32x32(my_s, t[0]);
-          tmem_ld_32x32(my_s + 32, t[1]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse),
-                              (e & 7) < kPolyPairs);
-        }
         // the memory of P served the last step's epilogue, of other warps too
         if (n > 0 && !(ok = warp_wait(epi_done, (n - 1) & 1, abort_flag))) break;
         // 16-byte piece u of a query's 64 keys lies at u ^ (query & 7), as TMA would have put it
@@ -302,63 +294,88 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           *reinterpret_cast<uint4*>(tile + sub * kChunkBytes + r * 128 + ((piece ^ (r & 7)) << 4)) =
               make_uint4(pk[0], pk[1], pk[2], pk[3]);
         };
-        if (active) {
+        auto probability = [&](const uint32_t(&x)[16], int e) {
+          return exp2_pair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, minus_lse), e < kPolyPairs);
+        };
+        auto put_chunk = [&](uint8_t* tile, uint32_t(&pk)[8], int c) {
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pk[e] &= keep_below(limit - 2 * (c * 8 + e));
+          }
+          put(tile, pk, c * 2);
+          put(tile, pk + 4, c * 2 + 1);
+        };
+        if (active && zeros) {
+          const uint32_t none[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            uint32_t pk[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 v = both(pr[c * 4 + e]);
-              pk[e] = pack_bf16(v.x, v.y) & keep_below(limit - 2 * (c * 4 + e));
-            }
-            put(sP, pk, c);
+            put(sP, none, c);
+            put(sDS, none, c);
           }
+        } else if (active) {
+          by_chunks(my_s, [&](int c, const uint32_t(&x)[16]) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 v = both(probability(x, e));
+              pk[e] = pack_bf16(v.x, v.y);
+            }
+            put_chunk(sP, pk, c);
+          });
         }
         tc_fence_before_sync();
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
-        if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
+        // delta, while dP is formed
+        if (!(ok = warp_wait(do_full, n & 1, abort_flag))) break;
+        row_dots<D, kCount>(sDO, y, dot_first, piece_u, s_delta + (n & 1) * 128);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(delta_ready);
+        if (!(ok = warp_wait(delta_ready, n & 1, abort_flag) && warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
-        if (active)
-          by_chunks(my_dp, [&](int c, const uint32_t(&x)[16]) {
+        if (active && !zeros) {
+          const float delta = row_ok ? s_delta[(n & 1) * 128 + r] : 0.f;
+          const f32x2 minus_delta = pair(-delta, -delta);
+          // P once more, from S, which is still there: kept, it would take the registers of the tables
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              uint32_t pk[4];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[16], d[16], pk[8];
+            tmem_ld_32x16(my_s + c * 16, x);
+            tmem_ld_32x16(my_dp + c * 16, d);
+            tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int v = half * 4 + e;
-                const float2 d = both(mul2(pr[c * 8 + v], add2(pair(__uint_as_float(x[2 * v]), __uint_as_float(x[2 * v + 1])), minus_delta)));
-                pk[e] = pack_bf16(d.x, d.y) & keep_below(limit - 2 * (c * 8 + v));
-              }
-              put(sDS, pk, c * 2 + half);
+            for (int e = 0; e < 8; ++e) {
+              const float2 v = both(mul2(probability(x, e), add2(pair(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1])), minus_delta)));
+              pk[e] = pack_bf16(v.x, v.y);
             }
-          });
+            put_chunk(sDS, pk, c);
+          }
+        }
         tc_fence_before_sync();
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
-        // dQ, and after the last head dK and dV: one copy of the code for the three
-        const int outputs = g + 1 < G ? 1 : (p.split > 1 ? 1 : 3);
-#pragma unroll 1
-        for (int which = 0; which < outputs; ++which) {
-          Turn<D> turn(p, first, which < 2 ? rows : 0, sub, lane);  // dV is not turned
-          if (kTurn) turn.fetch(0);
-          if (which == 0) {
-            if (!(ok = warp_wait(done, n & 1, abort_flag))) break;
-            tc_fence_after_sync();
-          }
-          __nv_bfloat16* base = which == 0 ? dq : (which == 1 ? dk : dv);
-          if (rows > 0)
-            write_rows<D, kTurn>((which == 0 ? tDP : (which == 1 ? tDK : tDV)) + lane_off, sub, which < 2 ? p.scale : 1.f, turn, rows,
-                                 stage, lane, base + row * p.out_stride + (which == 0 ? head0 + g : hkv) * D, p.out_stride);
-        }
+        if (g + 1 < G) fetch(h + 1);
+        else more = next_document();
         if (!ok) break;
-        if (g + 1 == G && p.split > 1 && rows > 0) {
-          const long long pitch = (long long)p.Hkv * D, size = p.T * pitch;
-          float* at = p.partial + part * 2 * size + row * pitch + hkv * D;
-          write_partial<D>(tDK + lane_off, sub, rows, stage, lane, at, pitch);
-          write_partial<D>(tDV + lane_off, sub, rows, stage, lane, at + size, pitch);
+        if (!(ok = warp_wait(done, n & 1, abort_flag))) break;
+        tc_fence_after_sync();
+        if (rows > 0) {
+          // dQ, and after the last head dK and dV: one copy of the code for the three
+          const int outputs = g + 1 < G || p.split > 1 ? 1 : 3;
+#pragma unroll 1
+          for (int which = 0; which < outputs; ++which) {
+            __nv_bfloat16* base = which == 0 ? dq : (which == 1 ? dk : dv);
+            write_rows_held<D, kTurn>((which == 0 ? tDP : (which == 1 ? tDK : tDV)) + lane_off, sub, which < 2 ? p.scale : 1.f, cs, sn,
+                                      which < 2, rows, stage, lane, base + row * p.out_stride + (which == 0 ? h : hkv0) * D, p.out_stride);
+          }
+          if (g + 1 == G && p.split > 1) {
+            const long long pitch = (long long)p.Hkv * D, size = p.T * pitch;
+            float* at = p.partial + part0 * 2 * size + row * pitch + hkv0 * D;
+            write_partial<D>(tDK + lane_off, sub, rows, stage, lane, at, pitch);
+            write_partial<D>(tDV + lane_off, sub, rows, stage, lane, at + size, pitch);
+          }
         }
         tc_fence_before_sync();
         __syncwarp();
@@ -373,7 +390,7 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 template <int D, bool kTurn>
 int launch_short_bwd(const CUtensorMap& tq, const CUtensorMap& tdo, const CUtensorMap& tk, const CUtensorMap& tv, BwdArgs p,
                      __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv, cudaStream_t stream) {
-  constexpr int SMEM = 5 * (D / 64) * kChunkBytes + 4 * kChunkBytes + 2560 + 320 + ItemRing::kBytes;
+  constexpr int SMEM = 5 * (D / 64) * kChunkBytes + 4 * kChunkBytes + 1024 + 320 + ItemRing::kBytes;
   static_assert(SMEM <= 232448, "one block's shared memory");
   constexpr auto kern = packed_short_bwd_kernel<D, kTurn>;
   if (cudaError_t e = pb::allow_smem<kern, SMEM>(); e != cudaSuccess) return (int)e;
