@@ -80,27 +80,11 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   return r;
 }
 
-// 2^x of a pair on the FMA pipe, where the special-function unit (16 results a clock and SM) is what bounds a softmax.
-// x = n + f with n the nearest integer, read from the low bits of x + 1.5 * 2^23; 2^f on [-1/2, 1/2] by the polynomial of
-// degree 4 whose largest relative error is least (2.7e-6 in fp32; the exchange algorithm of Remez); times 2^n by its
-// exponent bits.  x below -126 gives 2^-126 and not 0; NaN stays NaN.
-__device__ __forceinline__ f32x2 poly_exp2(f32x2 x) {
-  float2 v = both(x);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
-  x = pair(v.x, v.y);
-  const f32x2 t = add2(x, pair(12582912.f, 12582912.f));
-  const f32x2 n = add2(t, pair(-12582912.f, -12582912.f));
-  const f32x2 f = fma2(n, pair(-1.f, -1.f), x);
-  f32x2 p = pair(9.570102e-3f, 9.570102e-3f);
-  p = fma2(p, f, pair(5.591786e-2f, 5.591786e-2f));
-  p = fma2(p, f, pair(0.24024744f, 0.24024744f));
-  p = fma2(p, f, pair(0.6931218f, 0.6931218f));
-  p = fma2(p, f, pair(0.9999993f, 0.9999993f));
-  const float2 b = both(t);
-  const f32x2 e = pair(__uint_as_float((__float_as_uint(b.x) << 23) + 0x3f800000u),
-                       __uint_as_float((__float_as_uint(b.y) << 23) + 0x3f800000u));
-  return mul2(p, e);
+// One MUFU instruction each.  (A polynomial on the FMA pipe for a quarter or a half of them, degree 4 in pairs, was slower in
+// every kernel here: the softmax warps wait for their own chain of instructions, not for the special-function unit.)
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
+  const float2 v = both(x);
+  return pair(fast_exp2(v.x), fast_exp2(v.y));
 }
 
 // ------------------------------------------------------------------------------------------------ tiles

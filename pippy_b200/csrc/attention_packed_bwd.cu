@@ -303,8 +303,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (lane == 0) mbar_arrive(s_read);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse),
-                              (e & 7) < kPolyPairs);
+            pr[e] = exp2_pair(fma2(pair(__uint_as_float(t[e >> 4][(e & 15) * 2]), __uint_as_float(t[e >> 4][(e & 15) * 2 + 1])), scale2, minus_lse));
         }
         if (!(ok = warp_wait(dp_full, n & 1, abort_flag))) break;
         tc_fence_after_sync();
@@ -638,7 +637,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         by_chunks(my_s, [&](int c, const uint32_t(&x)[16]) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            pr[c * 8 + e] = exp2_pair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, pr[c * 8 + e]), e < kPolyPairs);
+            pr[c * 8 + e] = exp2_pair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, pr[c * 8 + e]));
         });
         // queries before this key are masked, in the packed results
         const bool masked = p.causal && blk == w.kv_tile;

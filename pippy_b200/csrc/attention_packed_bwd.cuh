@@ -26,15 +26,6 @@ struct BwdArgs {
   int* err;
 };
 
-// kPolyPairs of 8 pairs of exponentials are computed on the FMA pipe (poly_exp2)
-constexpr int kPolyPairs = 4;
-
-__device__ __forceinline__ f32x2 exp2_pair(f32x2 x, bool poly) {
-  if (poly) return poly_exp2(x);
-  const float2 v = both(x);
-  return pair(fast_exp2(v.x), fast_exp2(v.y));
-}
-
 // Mask of a packed pair of bf16 of which the first `n` values stay (all for n >= 2, none for n <= 0).
 __device__ __forceinline__ uint32_t keep_below(int n) {
   uint32_t m;

@@ -32,8 +32,6 @@ struct FwdArgs {
 };
 
 constexpr int kFwdThreads = 384;
-// kPolyPairsFwd of 8 pairs of exponentials are computed on the FMA pipe (poly_exp2)
-constexpr int kPolyPairsFwd = 2;
 
 template <int D>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -155,9 +153,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   int used[2] = {0, 0};  // items so far that had the tile
   int n = 0;             // K / V stages so far
-  // launched with 168 registers a thread: 72 + 2 x 216 = 3 x 168
+  // launched with 168 registers a thread: 88 + 2 x 208 = 3 x 168
   if (warp < 4) {
-    give_registers<72>();
+    give_registers<88>();
     if (warp == 0) {
     while (ok && publish_next()) {
       if (w.blocks[0] == 0) continue;
@@ -265,7 +263,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     }
   } else {
-    take_registers<216>();
+    take_registers<208>();
     // ------------------------------------------------------------ softmax + epilogue, one query row per thread
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
@@ -294,8 +292,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, v[c]);
         tmem_ld_wait();
-        const bool masked = (p.causal && k0 + 127 > first_row) || k0 + 128 > w.len;
-        if (masked) {
+        if ((p.causal && k0 + 127 > first_row) || k0 + 128 > w.len) {
           // keys this row may see: [k0, limit)
           const int limit = (p.causal ? min(w.len, q_idx + 1) : w.len) - k0;
 #pragma unroll
@@ -334,29 +331,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const f32x2 minus_m = pair(-m, -m);
         f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
         // P over the first 64 columns of S, which is in registers by now
-        auto exponentials = [&](auto poly) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const f32x2 x = fma2(pair(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), scale2, minus_m);
-              f32x2 y;
-              if (decltype(poly)::value && (e & 7) < kPolyPairsFwd) {
-                y = poly_exp2(x);
-              } else {
-                const float2 b = both(x);
-                y = pair(fast_exp2(b.x), fast_exp2(b.y));
-              }
-              sum[e & 1] = add2(sum[e & 1], y);
-              const float2 b = both(y);
-              pk[e] = pack_bf16(b.x, b.y);
-            }
-            tmem_st_32x16(tS + c * 16, pk);
+          for (int e = 0; e < 16; ++e) {
+            const f32x2 y = exp2_pair(fma2(pair(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), scale2, minus_m));
+            sum[e & 1] = add2(sum[e & 1], y);
+            const float2 b = both(y);
+            pk[e] = pack_bf16(b.x, b.y);
           }
-        };
-        if (masked) exponentials(Flag<false>{});  // a masked score has to give 0 exactly
-        else exponentials(Flag<true>{});
+          tmem_st_32x16(tS + c * 16, pk);
+        }
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();

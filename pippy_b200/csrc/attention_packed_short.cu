@@ -19,6 +19,8 @@ namespace pbv {
 
 constexpr int kShortThreads = 384;
 
+__device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
+
 template <int D, bool kTurn>
 __global__ void __launch_bounds__(kShortThreads, 1)
 packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -157,7 +159,7 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       };
       while (ok && next_item()) {
         if (pad) continue;
-        const int n16 = (len + 15) & ~15, steps = n16 >> 4;
+        const int n16 = up16(len), steps = n16 >> 4;
         const uint32_t idesc_s = make_idesc_bf16(128, n16, 0, 0);
         if (!(ok = wait(k_full, it & 1) && wait(v_full, it & 1))) break;
         for (int g = 0; g < G; ++g, ++n) {
@@ -195,7 +197,7 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       auto clear = [&](uint8_t* tile, uint64_t* raw, int bit, uint64_t* full) {
         if (!warp_wait(raw, (phases >> bit) & 1, abort_flag)) return false;
         phases ^= 1u << bit;
-        const int bytes = (((len + 15) & ~15) - len) * 128;
+        const int bytes = (up16(len) - len) * 128;
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
           for (int at = lane * 16; at < bytes; at += 512)
@@ -273,7 +275,7 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     bool more = next_document();
     while (ok && more) {
       const int head0 = (hkv * p.split + part) * G, hkv0 = hkv, part0 = part;
-      const int n16 = (len + 15) & ~15;
+      const int n16 = up16(len);
       // which of its scores a product reads, and which of these are not masked
       const bool active = quarter * 32 < n16 && sub * 64 < n16;
       const bool zeros = p.causal && sub * 64 > quarter * 32 + 31;
@@ -295,7 +297,7 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
               make_uint4(pk[0], pk[1], pk[2], pk[3]);
         };
         auto probability = [&](const uint32_t(&x)[16], int e) {
-          return exp2_pair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, minus_lse), e < kPolyPairs);
+          return exp2_pair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, minus_lse));
         };
         auto put_chunk = [&](uint8_t* tile, uint32_t(&pk)[8], int c) {
           if (masked) {
