@@ -295,11 +295,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if ((p.causal && k0 + 127 > first_row) || k0 + 128 > w.len) {
           // keys this row may see: [k0, limit)
           const int limit = (p.causal ? min(w.len, q_idx + 1) : w.len) - k0;
+          // as bits: a test of a bit of a register that every element shares is cheaper than a comparison
+          uint32_t seen[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int n = min(max(limit - c * 32, 0), 32);
+            seen[c] = n == 32 ? 0xffffffffu : (1u << n) - 1;
+          }
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (c * 32 + e >= limit) v[c][e] = 0xff800000u;  // -inf
+              if (!((seen[c] >> e) & 1)) v[c][e] = 0xff800000u;  // -inf
         }
         float mx[4];  // four chains: one would be 128 dependent steps
 #pragma unroll
@@ -314,7 +321,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const float m_use = (m_cand == -CUDART_INF_F) ? 0.f : m_cand;
           const float alpha = exp2f(m - m_use);  // 0 on the first block (m = -inf)
           if (j > 0) {
-#pragma unroll
+#pragma unroll 1  // rare: its code should not push the rest out of the instruction cache
             for (int cc = 0; cc < D / 16; ++cc) {  // 16 columns at a time: v is live
               uint32_t o[16];
               tmem_ld_32x16(tO + cc * 16, o);
