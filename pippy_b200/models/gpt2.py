@@ -15,8 +15,8 @@ import torch.distributed as dist
 import torch.nn as nn
 
 from ..ops import functional as pf
-from .layers import Embedding, LayerNorm, Linear
-from .llama import layer_range
+from .layers import Dropout, Embedding, LayerNorm, Linear
+from .llama import batch_layout, layer_range
 
 
 @dataclass
@@ -29,6 +29,8 @@ class GPT2Config:
     norm_eps: float = 1e-5
     init_std: float = 0.02
     vocab_multiple: int = 128  # the embedding / head are padded to a multiple of this many rows
+    dropout: float = 0.0  # of the embeddings and of both residual branches of a block, in training
+    sorted_embedding_grad: bool = False  # the tables' gradients in token order, the same bits on every run
 
     @property
     def padded_vocab(self) -> int:
@@ -54,9 +56,10 @@ class GPT2Config:
 
 
 class GPT2Block(nn.Module):
-    def __init__(self, cfg: GPT2Config, device=None, dtype=None):
+    def __init__(self, cfg: GPT2Config, device=None, dtype=None, index: int = 0):
         super().__init__()
-        self.cfg = cfg
+        self.cfg, self.index = cfg, index
+        self.drop = Dropout(cfg.dropout)
         d = cfg.dim
         self.ln_1 = LayerNorm(d, cfg.norm_eps, device=device, dtype=dtype)
         self.attn_c_attn = Linear(d, 3 * d, bias=True, init_std=cfg.init_std, device=device, dtype=dtype)
@@ -65,26 +68,40 @@ class GPT2Block(nn.Module):
         self.mlp_c_fc = Linear(d, 4 * d, bias=True, init_std=cfg.init_std, device=device, dtype=dtype)
         self.mlp_c_proj = Linear(4 * d, d, bias=True, init_std=cfg.init_std, device=device, dtype=dtype)
 
-    def forward(self, x, B: int, S: int):
+    def forward(self, x, B: int, S: int, layout=None, seed=None):
+        """``layout``: documents in the rows.  ``seed``: of the stage's dropout masks; the block's index tells them apart."""
         cfg = self.cfg
         qkv = self.attn_c_attn(self.ln_1(x))
-        att = pf.rope_attention(qkv, None, None, B, S, cfg.n_heads, cfg.n_heads, cfg.head_dim)
-        x = self.attn_c_proj(att, residual=x)
+        if layout is None:
+            att = pf.rope_attention(qkv, None, None, B, S, cfg.n_heads, cfg.n_heads, cfg.head_dim)
+        else:
+            att = pf.packed_attention(qkv, None, None, layout, cfg.n_heads, cfg.n_heads, cfg.head_dim)
+        if seed is None:
+            x = self.attn_c_proj(att, residual=x)
+        else:
+            x = self.drop(self.attn_c_proj(att), residual=x, seed=seed, stream=2 * self.index + 1)
         h = self.mlp_c_fc(self.ln_2(x), activation="gelu_tanh")
-        return self.mlp_c_proj(h, residual=x)
+        if seed is None:
+            return self.mlp_c_proj(h, residual=x)
+        return self.drop(self.mlp_c_proj(h), residual=x, seed=seed, stream=2 * self.index + 2)
 
 
 class GPT2Stage(nn.Module):
     """Input: token ids [B, S] (first stage) or hidden states [B, S, dim]; output: hidden states or logits
-    [B, S, padded_vocab]."""
+    [B, S, padded_vocab].
+
+    ``lengths`` ([B, documents], see ``pf.packed_layout``): the rows hold documents, which do not see one another and
+    whose positions begin at 0; every stage gets it.  With ``cfg.dropout`` a training forward draws one seed from the
+    device's default generator (data-parallel ranks seed theirs differently)."""
 
     def __init__(self, cfg: GPT2Config, layer_ids, first: bool, last: bool, device=None, dtype=None):
         super().__init__()
         self.cfg, self.first, self.last = cfg, first, last
         if first:
             self.wte = Embedding(cfg.padded_vocab, cfg.dim, max_positions=cfg.n_positions, init_std=cfg.init_std,
-                                 device=device, dtype=dtype)
-        self.h = nn.ModuleDict({str(i): GPT2Block(cfg, device=device, dtype=dtype) for i in layer_ids})
+                                 device=device, dtype=dtype, sorted_grad=cfg.sorted_embedding_grad)
+        self.drop = Dropout(cfg.dropout)
+        self.h = nn.ModuleDict({str(i): GPT2Block(cfg, device=device, dtype=dtype, index=int(i)) for i in layer_ids})
         if last:
             self.ln_f = LayerNorm(cfg.dim, cfg.norm_eps, device=device, dtype=dtype)
             if first:
@@ -95,15 +112,18 @@ class GPT2Stage(nn.Module):
     def head_weight(self) -> torch.Tensor:
         return self.wte.weight if self.first else self.lm_head.weight
 
-    def forward(self, x):
+    def forward(self, x, lengths=None):
+        B, S = x.shape[:2]
+        layout = None if lengths is None else batch_layout(lengths, B, S)
+        seed = Dropout.draw(x.device) if self.training and self.cfg.dropout > 0.0 else None
         if self.first:
-            B, S = x.shape
-            h = self.wte(x)
+            h = self.wte(x, None if layout is None else layout.positions)
+            if seed is not None:
+                h = self.drop(h, seed=seed)
         else:
-            B, S, _ = x.shape
             h = x.reshape(B * S, -1)
         for blk in self.h.values():
-            h = blk(h, B, S)
+            h = blk(h, B, S, layout, seed)
         if self.last:
             h = pf.linear(self.ln_f(h), self.head_weight())
         return h.view(B, S, -1)

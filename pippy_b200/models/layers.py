@@ -60,11 +60,39 @@ class LayerNorm(nn.Module):
         return pf.layer_norm(x, self.weight, self.bias, self.eps)
 
 
-class Embedding(nn.Module):
-    """Token embedding with an optional learned position table; returns ``[B*S, H]``."""
+class Dropout(nn.Module):
+    """``pf.dropout`` in training, with a seed drawn from the device's default generator (so that ``torch.manual_seed`` and
+    activation checkpointing, which replays that generator, govern the mask); the identity in evaluation.  ``residual`` is
+    added in the same pass."""
 
-    def __init__(self, vocab: int, dim: int, max_positions: int = 0, init_std: float = 0.02, device=None, dtype=None):
+    def __init__(self, p: float):
         super().__init__()
+        if not 0.0 <= p < 1.0:
+            raise ValueError(f"dropout probability {p}")
+        self.p = p
+
+    def forward(self, x, residual=None, seed=None, stream: int = 0):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else x + residual
+        return pf.dropout(x, self.p, self.draw(x.device) if seed is None else seed, residual=residual, stream=stream)
+
+    @staticmethod
+    def draw(device) -> torch.Tensor:
+        """A seed for :func:`pf.dropout`; layers that share one pass a ``stream`` each."""
+        return torch.empty(1, dtype=torch.int64, device=device).random_()
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}"
+
+
+class Embedding(nn.Module):
+    """Token embedding, times ``scale``, with an optional learned position table; returns ``[B*S, H]``.  ``sorted_grad``: see
+    ``pf.embedding``."""
+
+    def __init__(self, vocab: int, dim: int, max_positions: int = 0, init_std: float = 0.02, device=None, dtype=None,
+                 scale: float = 1.0, sorted_grad: bool = False):
+        super().__init__()
+        self.scale, self.sorted_grad = scale, sorted_grad
         self.weight = nn.Parameter(torch.empty(vocab, dim, device=device, dtype=dtype))
         self.positions = (
             nn.Parameter(torch.empty(max_positions, dim, device=device, dtype=dtype)) if max_positions > 0 else None
@@ -74,13 +102,15 @@ class Embedding(nn.Module):
             if self.positions is not None:
                 nn.init.normal_(self.positions, std=init_std)
 
-    def forward(self, ids):
+    def forward(self, ids, positions=None):
+        """``positions``: each token's own (a ``pf.PackedLayout``'s), instead of its place in the row."""
         S = ids.shape[-1]
         wpe = self.positions[:S] if self.positions is not None and self.positions.shape[0] != S else self.positions
         if wpe is not None and wpe is not self.positions:
             # a sliced view would lose the parameter identity the gradient is written to; use the full table
             wpe = self.positions
-        return pf.embedding(ids, self.weight, wpe, S)
+        return pf.embedding(ids, self.weight, wpe, S, scale=self.scale, positions=None if wpe is None else positions,
+                            sorted_grad=self.sorted_grad)
 
 
 class RotaryCache:

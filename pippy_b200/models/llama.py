@@ -86,14 +86,17 @@ class LlamaAttention(nn.Module):
         if has_out:
             self.wo = Linear(cfg.n_heads * hd, cfg.dim, init_std=cfg.init_std, device=device, dtype=dtype)
 
-    def core(self, h, B: int, S: int):
+    def core(self, h, B: int, S: int, layout=None):
+        """``layout`` (``pf.PackedLayout``): attention and positions per document instead of per row."""
         cfg = self.cfg
         qkv = self.wqkv(h)
         cos, sin = ROTARY.get(S, cfg.head_dim, cfg.rope_theta, h.device)
+        if layout is not None:
+            return pf.packed_attention(qkv, cos, sin, layout, cfg.n_heads, cfg.kv_heads, cfg.head_dim, inplace=True)
         return pf.rope_attention(qkv, cos, sin, B, S, cfg.n_heads, cfg.kv_heads, cfg.head_dim)
 
-    def forward(self, h, residual, B: int, S: int):
-        return self.wo(self.core(h, B, S), residual=residual)
+    def forward(self, h, residual, B: int, S: int, layout=None):
+        return self.wo(self.core(h, B, S, layout), residual=residual)
 
 
 class LlamaMLP(nn.Module):
@@ -140,7 +143,7 @@ class LlamaBlock(nn.Module):
             self.feed_forward = LlamaMLP(cfg, device=device, dtype=dtype, has_gate_up="f1" in units,
                                          has_down="f2" in units)
 
-    def forward(self, x, B: int, S: int, carry=None):
+    def forward(self, x, B: int, S: int, carry=None, layout=None):
         """``x``: residual stream ``[B*S, dim]``; ``carry``: the attention output or the SwiGLU output handed over
         by the previous stage when this block starts at a2 or f2.  Returns ``x`` (or ``(x, carry)`` when the block
         ends at a1 or f1)."""
@@ -149,7 +152,7 @@ class LlamaBlock(nn.Module):
         # added inside the norm-backward kernel
         if "a1" in u:
             n, x = self.attention_norm.fork(x)
-            carry = self.attention.core(n, B, S)
+            carry = self.attention.core(n, B, S, layout)
         if "a2" in u:
             x, carry = self.attention.wo(carry, residual=x), None
         if "f1" in u:
@@ -158,6 +161,13 @@ class LlamaBlock(nn.Module):
         if "f2" in u:
             x, carry = self.feed_forward.w_down(carry, residual=x), None
         return x if carry is None else (x, carry)
+
+
+def batch_layout(lengths, B: int, S: int) -> "pf.PackedLayout":
+    """The layout of a ``[B, S]`` batch whose row ``b`` holds documents of ``lengths[b]`` tokens."""
+    if lengths.dim() != 2 or lengths.shape[0] != B:
+        raise ValueError(f"lengths: [{B}, documents] for {B} rows, got {tuple(lengths.shape)}")
+    return pf.packed_layout(lengths, S)
 
 
 def layer_range(n_layers: int, stage: int, num_stages: int) -> range:
@@ -293,7 +303,10 @@ class LlamaStage(nn.Module):
     only part of (see :class:`LlamaBlock`); the embedding goes with ``first`` and the final norm + head with
     ``last``.  Input: token ids ``[B, S]`` (first stage) or hidden states ``[B, S, dim]``, plus a second tensor
     ``[B, S, dim or ffn_dim]`` when the stage starts in the middle of an attention or MLP half; output: hidden states
-    (plus such a second tensor when it ends in the middle of one) or logits ``[B, S, vocab]``."""
+    (plus such a second tensor when it ends in the middle of one) or logits ``[B, S, vocab]``.
+
+    ``lengths`` (``[B, documents]``, see ``pf.packed_layout``): the rows hold documents, which do not see one another; every
+    stage gets it, through ``stage_kwargs`` of the schedule's ``step``."""
 
     def __init__(self, cfg: LlamaConfig, layer_ids, first: bool, last: bool, device=None, dtype=None,
                  activation_checkpointing: bool = False):
@@ -317,7 +330,7 @@ class LlamaStage(nn.Module):
         self.carry_in = 0 if first else {"a2": carry_dim["a1"], "f2": carry_dim["f1"]}.get(first_unit, 0)
         self.carry_out = 0 if last else carry_dim.get(last_unit, 0)
 
-    def forward(self, x, carry=None):
+    def forward(self, x, carry=None, lengths=None):
         if self.first:
             B, S = x.shape
             h = self.tok_embeddings(x)
@@ -326,14 +339,17 @@ class LlamaStage(nn.Module):
             h = x.reshape(B * S, -1)
             if carry is not None:
                 carry = carry.reshape(B * S, -1)
+        layout = None
+        if lengths is not None and any("a1" in blk.units for blk in self.layers.values()):
+            layout = batch_layout(lengths, B, S)
         recompute = self.activation_checkpointing and torch.is_grad_enabled() and h.requires_grad
         for blk in self.layers.values():
             if recompute:
                 # keep only the block's input; its forward runs again inside the backward (the reference lists
                 # activation checkpointing as a TODO, ARCHITECTURE.md:201).  Costs one extra forward per block.
-                out = torch.utils.checkpoint.checkpoint(blk, h, B, S, carry, use_reentrant=False)
+                out = torch.utils.checkpoint.checkpoint(blk, h, B, S, carry, layout, use_reentrant=False)
             else:
-                out = blk(h, B, S, carry)
+                out = blk(h, B, S, carry, layout)
             h, carry = out if isinstance(out, tuple) else (out, None)
         if self.last:
             h = self.output(self.norm(h))

@@ -17,7 +17,7 @@ import torch.nn as nn
 from ..ops import functional as pf
 from ..parallel.tp import ColumnParallelLinear, RowParallelLinear, TPContext
 from .layers import ROTARY, Embedding, Linear, RMSNorm
-from .llama import LlamaConfig, layer_range
+from .llama import LlamaConfig, batch_layout, layer_range
 
 
 class _GatherForHead(torch.autograd.Function):
@@ -56,11 +56,14 @@ class TPLlamaBlock(nn.Module):
         self.w_gate_up = ColumnParallelLinear(cfg.dim, 2 * cfg.ffn_dim, tp, tp_size, cfg.init_std, device=device, dtype=dtype)
         self.w_down = RowParallelLinear(cfg.ffn_dim, cfg.dim, tp, tp_size, cfg.init_std, device=device, dtype=dtype)
 
-    def forward(self, x_shard, B: int, S: int):
+    def forward(self, x_shard, B: int, S: int, layout=None):
         cfg = self.cfg
         qkv = self.wqkv(self.attention_norm(x_shard))  # [T, (hq + 2 hkv) * hd] for this rank's heads
         cos, sin = ROTARY.get(S, cfg.head_dim, cfg.rope_theta, x_shard.device)
-        att = pf.rope_attention(qkv, cos, sin, B, S, self.hq, self.hkv, cfg.head_dim)
+        if layout is None:
+            att = pf.rope_attention(qkv, cos, sin, B, S, self.hq, self.hkv, cfg.head_dim)
+        else:
+            att = pf.packed_attention(qkv, cos, sin, layout, self.hq, self.hkv, cfg.head_dim, inplace=True)
         x_shard = self.wo(att, x_shard)                # reduce-scatter + residual
         h = pf.swiglu(self.w_gate_up(self.ffn_norm(x_shard)))
         return self.w_down(h, x_shard)
@@ -83,7 +86,8 @@ class TPLlamaStage(nn.Module):
             self.norm = RMSNorm(cfg.dim, cfg.norm_eps, device=device, dtype=dtype)
             self.output = Linear(cfg.dim, cfg.vocab_size, init_std=cfg.init_std, device=device, dtype=dtype)
 
-    def forward(self, x):
+    def forward(self, x, lengths=None):
+        """``lengths`` as in :class:`.llama.LlamaStage`, the same on every tensor-parallel rank."""
         B, S = self.B, self.S
         rows = B * S // self.tp_size
         if self.first:
@@ -91,8 +95,9 @@ class TPLlamaStage(nn.Module):
             h = self.tok_embeddings(flat.view(1, -1))
         else:
             h = x
+        layout = None if lengths is None or not self.layers else batch_layout(lengths, B, S)
         for blk in self.layers.values():
-            h = blk(h, B, S)
+            h = blk(h, B, S, layout)
         if self.last:
             h = self.norm(h)
             if self.tp_size > 1:

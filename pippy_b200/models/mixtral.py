@@ -14,7 +14,7 @@ import torch.nn as nn
 from ..ops import functional as pf
 from ..parallel.ep import EPContext, MoEFeedForward
 from .layers import Embedding, Linear, RMSNorm
-from .llama import LlamaAttention, LlamaConfig, layer_range
+from .llama import LlamaAttention, LlamaConfig, batch_layout, layer_range
 
 
 @dataclass
@@ -43,8 +43,8 @@ class MixtralBlock(nn.Module):
         self.block_sparse_moe = MoEFeedForward(cfg.dim, cfg.ffn_dim, cfg.n_experts, cfg.top_k, ep, ep_size, ep_rank,
                                                cfg.aux_coef, cfg.init_std, device=device, dtype=dtype)
 
-    def forward(self, x, B: int, S: int):
-        x = self.attention(self.attention_norm(x), x, B, S)
+    def forward(self, x, B: int, S: int, layout=None):
+        x = self.attention(self.attention_norm(x), x, B, S, layout)
         return x + self.block_sparse_moe(self.ffn_norm(x))
 
 
@@ -62,15 +62,17 @@ class MixtralStage(nn.Module):
             self.norm = RMSNorm(cfg.dim, cfg.norm_eps, device=device, dtype=dtype)
             self.output = Linear(cfg.dim, cfg.vocab_size, init_std=cfg.init_std, device=device, dtype=dtype)
 
-    def forward(self, x):
+    def forward(self, x, lengths=None):
+        """``lengths`` as in :class:`.llama.LlamaStage`."""
         if self.first:
             B, S = x.shape
             h = self.tok_embeddings(x)
         else:
             B, S, _ = x.shape
             h = x.reshape(B * S, -1)
+        layout = None if lengths is None or not self.layers else batch_layout(lengths, B, S)
         for blk in self.layers.values():
-            h = blk(h, B, S)
+            h = blk(h, B, S, layout)
         if self.last:
             h = self.output(self.norm(h))
         return h.view(B, S, -1)

@@ -247,6 +247,8 @@ class PipelineSchedule:
             raise TypeError(f"losses must be a list but got a {type(losses)}")
         return arg_mbs, kwarg_mbs
 
+    _shared_kwarg_mbs: Optional[List[Dict[str, Any]]] = None  # keyword arguments of every stage, per microbatch, during a step
+
     def _split_inputs(self, args: Tuple[Any, ...], kwargs: Optional[Dict[str, Any]]):
         if args or kwargs:
             args_split, kwargs_split = split_args_kwargs_into_chunks(
@@ -302,6 +304,7 @@ class PipelineSchedule:
 
     def _step_microbatches(self, arg_mbs=None, kwarg_mbs=None, target_mbs=None, losses=None) -> None:
         arg_mbs, kwarg_mbs = self._check_inputs(arg_mbs, kwarg_mbs, target_mbs, losses)
+        shared = self._shared_kwarg_mbs or [{}] * self._n_microbatches
         if self._actions is None:
             self._build()
         stages = self._stage_by_index
@@ -338,9 +341,9 @@ class PipelineSchedule:
                 t0 = timer.start() if timer else None
                 with record_function(f"Forward {mb}" if self._num_local == 1 else f"Stage {action.stage} Forward {mb}"):
                     if st.is_first:
-                        out = st.forward_one_chunk(mb, arg_mbs[mb], kwarg_mbs[mb])
+                        out = st.forward_one_chunk(mb, arg_mbs[mb], {**kwarg_mbs[mb], **shared[mb]})
                     else:
-                        out = st.forward_one_chunk(mb, (), {})
+                        out = st.forward_one_chunk(mb, (), shared[mb])
                     out_tuple = out if isinstance(out, tuple) else (out,)
                     for out_idx, dst in st.local_forward_targets():
                         stages[dst].set_local_input(mb, st.stage_index, out_idx, out_tuple[out_idx])
@@ -388,12 +391,16 @@ class PipelineSchedule:
         self._update_losses(losses)
 
     # ------------------------------------------------------------------ public
-    def step(self, *args, target=None, losses: Optional[List] = None, **kwargs):
+    def step(self, *args, target=None, losses: Optional[List] = None, stage_kwargs: Optional[Dict[str, Any]] = None,
+             **kwargs):
         """Runs one full batch through the pipeline.
 
         The rank holding the first stage passes the model inputs, the rank holding the last stage passes
         ``target`` (when a loss function is set) and may pass a ``losses`` list to receive the per-microbatch
         losses; it gets the merged output back. Every other rank calls ``step()`` and gets ``None``.
+
+        ``kwargs`` go to the first stage. ``stage_kwargs`` go to every stage's forward (document lengths of packed rows,
+        say), split along their first dimension like the inputs; every rank passes the same.
         """
         for st in self._stages:
             st.clear_runtime_states()
@@ -404,7 +411,14 @@ class PipelineSchedule:
             targets_split = list(torch.tensor_split(target, self._n_microbatches))
         else:
             targets_split = None
-        self._step_microbatches(args_split, kwargs_split, targets_split, losses)
+        if stage_kwargs:
+            _, self._shared_kwarg_mbs = split_args_kwargs_into_chunks((), stage_kwargs, self._n_microbatches)
+            if len(self._shared_kwarg_mbs) != self._n_microbatches:
+                raise ValueError(f"stage_kwargs: {self._n_microbatches} microbatches do not come out of their first dimension")
+        try:
+            self._step_microbatches(args_split, kwargs_split, targets_split, losses)
+        finally:
+            self._shared_kwarg_mbs = None
         if not self.return_outputs:
             return None
         for st in self._stages:

@@ -48,15 +48,20 @@ class Pipeline:
     tied: Any = None
     pre_optimizer: List[Callable[[], None]] = field(default_factory=list)  # run after the schedule, before the update
 
-    def train_step(self, inputs=None, target=None) -> Optional[torch.Tensor]:
+    def train_step(self, inputs=None, target=None, lengths=None) -> Optional[torch.Tensor]:
         """One optimizer step over one global batch. The rank holding the first stage passes ``inputs``, the rank
-        holding the last stage passes ``target`` and gets the mean loss (a device scalar) back."""
+        holding the last stage passes ``target`` and gets the mean loss (a device scalar) back.
+
+        ``lengths`` (``[global batch, documents]``, every rank passes the same): the rows hold documents one after the
+        other, which do not see one another; a length of 0 is no document, and what a row has left is padding, whose
+        targets should be the loss's ``ignore_index``."""
         self.losses.clear()
         args = (inputs,) if self.holds_first and inputs is not None else ()
+        packed = {} if lengths is None else {"stage_kwargs": {"lengths": lengths}}
         if self.holds_last:
-            self.schedule.step(*args, target=target, losses=self.losses)
+            self.schedule.step(*args, target=target, losses=self.losses, **packed)
         else:
-            self.schedule.step(*args)
+            self.schedule.step(*args, **packed)
         if self.tied is not None:
             self.tied.sync_grads()
         for hook in self.pre_optimizer:

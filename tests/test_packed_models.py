@@ -1,0 +1,263 @@
+"""Models on packed documents: a packed batch gives what its documents give one by one."""
+import pytest
+import torch
+
+from _mp import run_ranks
+
+LENGTHS = [[5, 0, 7, 3], [16, 0, 0, 0], [1, 1, 9, 4]]
+S = 16
+
+
+def _documents(ids, lengths):
+    for row, counts in zip(ids, lengths):
+        at = 0
+        for n in counts:
+            if n:
+                yield row[at : at + n].unsqueeze(0)
+            at += n
+
+
+def _inside(lengths):
+    return torch.tensor([[t < sum(row) for t in range(S)] for row in lengths])
+
+
+def _llama(dtype):
+    from pippy_b200.models.llama import Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    return Llama(LlamaConfig.tiny(vocab_size=64, dim=32, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=48), dtype=dtype)
+
+
+def _gpt2(dtype, **kw):
+    from pippy_b200.models.gpt2 import GPT2Config, GPT2Stage
+
+    torch.manual_seed(0)
+    cfg = GPT2Config(vocab_size=60, n_positions=S, dim=32, n_layers=2, n_heads=2, vocab_multiple=8, **kw)
+    return GPT2Stage(cfg, range(2), True, True, dtype=dtype)
+
+
+def _mixtral(dtype):
+    from pippy_b200.models.mixtral import MixtralConfig, MixtralStage
+
+    torch.manual_seed(0)
+    cfg = MixtralConfig(vocab_size=64, dim=32, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=48, n_experts=4, aux_coef=0.0)
+    return MixtralStage(cfg, range(2), True, True, dtype=dtype)
+
+
+def _tp(dtype):
+    from pippy_b200.models.llama import LlamaConfig
+    from pippy_b200.models.llama_tp import TPLlamaStage
+
+    torch.manual_seed(0)
+    cfg = LlamaConfig.tiny(vocab_size=64, dim=32, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=48)
+    return TPLlamaStage(cfg, range(2), True, True, None, 1, 0, len(LENGTHS), S, dtype=dtype)
+
+
+@pytest.mark.parametrize("build", [_llama, _gpt2, _mixtral, _tp])
+def test_packed_batch_equals_its_documents(build):
+    model = build(torch.float64)
+    ids = torch.randint(0, 60, (3, S), generator=torch.Generator().manual_seed(1))
+    lengths = torch.tensor(LENGTHS)
+    inside = _inside(LENGTHS)
+    g = torch.randn(int(inside.sum()), 64, dtype=torch.float64, generator=torch.Generator().manual_seed(2))
+    out = model(ids, lengths=lengths)[inside]
+    packed = torch.autograd.grad(out, list(model.parameters()), g)
+    if build is _tp:  # a module of one shape: each document alone in its row
+        alone = []
+        for b, d in enumerate(_documents(ids, LENGTHS)):
+            rows = torch.zeros(3, S, dtype=torch.int64)
+            rows[0, : d.shape[1]] = d
+            alone.append(model(rows)[0, : d.shape[1]])
+        alone = torch.cat(alone)
+    else:
+        alone = torch.cat([model(d)[0] for d in _documents(ids, LENGTHS)])
+    # fp32 inside the plain norms and attention of the dense path: 2^-24 of sums of some tens of terms, a few layers deep
+    assert torch.allclose(out, alone, rtol=1e-4, atol=1e-6)
+    for a, b in zip(packed, torch.autograd.grad(alone, list(model.parameters()), g)):
+        assert torch.allclose(a, b, rtol=1e-3, atol=1e-5)
+    with pytest.raises(ValueError):
+        model(ids, lengths=lengths[:2])
+
+
+def test_recomputation_keeps_the_layout():
+    from pippy_b200.models.llama import LlamaConfig, LlamaStage
+
+    cfg = LlamaConfig.tiny(vocab_size=64, dim=32, n_layers=2, n_heads=4, ffn_dim=48)
+    ids, lengths = torch.randint(0, 64, (3, S), generator=torch.Generator().manual_seed(1)), torch.tensor(LENGTHS)
+    grads = []
+    for again in (False, True):
+        torch.manual_seed(0)
+        model = LlamaStage(cfg, range(2), True, True, dtype=torch.float64, activation_checkpointing=again)
+        model(ids, lengths=lengths)[_inside(LENGTHS)].square().sum().backward()
+        grads.append([p.grad for p in model.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_dropout_of_gpt2():
+    """Reproducible under a seed, another mask otherwise, nothing in evaluation; the gradient is that of the same masks."""
+    model = _gpt2(torch.float64, dropout=0.2)
+    plain = _gpt2(torch.float64)
+    ids = torch.randint(0, 60, (2, S), generator=torch.Generator().manual_seed(1))
+
+    def run(seed):
+        torch.manual_seed(seed)
+        return model(ids)
+
+    assert torch.equal(run(1), run(1)) and not torch.equal(run(1), run(2))
+    w = model.h["1"].mlp_c_fc.weight
+    direction = torch.randn(w.shape, dtype=w.dtype, generator=torch.Generator().manual_seed(3))
+    (grad,) = torch.autograd.grad(run(1).square().sum(), w)
+    step = 1e-3
+    with torch.no_grad():
+        w += step * direction
+        up = run(1).square().sum()
+        w -= 2 * step * direction
+        down = run(1).square().sum()
+        w += step * direction
+    # the difference's error is step^2 of the third derivative; norms run in 32 bits: 2^-24 of the sum over 2 step
+    assert abs((up - down) / (2 * step) - (grad * direction).sum()) < 1e-2 * abs((grad * direction).sum()) + 1e-3
+    model.eval()
+    plain.load_state_dict(model.state_dict())
+    assert torch.equal(model(ids), plain(ids))
+
+
+def _train(rank, world, schedule):
+    import torch.distributed as dist
+
+    from pippy_b200.models.llama import LlamaConfig, causal_lm_loss
+    from pippy_b200.train import build_llama_pipeline
+
+    cfg = LlamaConfig.tiny(vocab_size=64, dim=32, n_layers=4, n_heads=4, ffn_dim=48)
+    lengths = torch.tensor(LENGTHS + [[2, 2, 0, 12]])
+    ids = torch.randint(0, 64, (4, S), generator=torch.Generator().manual_seed(1))
+    target = torch.where(torch.cat([_inside(LENGTHS), torch.ones(1, S, dtype=torch.bool)]), ids.roll(-1, 1), -100)
+    stages = 1 if schedule == "1f1b" else 2
+    pipe = build_llama_pipeline(cfg, 4, S, 2, torch.device("cpu"), schedule=schedule, virtual_stages=stages, dtype=torch.float64,
+                                lr=0.0, weight_decay=0.0)
+    loss = pipe.train_step(ids if pipe.holds_first else None, target if pipe.holds_last else None, lengths)
+    if not pipe.holds_last:
+        return
+    from pippy_b200.models.llama import build_llama_stage
+
+    n = stages * world
+    parts = []
+    for s in range(n):
+        torch.manual_seed(s)
+        parts.append(build_llama_stage(cfg, s, n, dtype=torch.float64, pp_size=world, seq_len=S))
+    want = []
+    for mb in range(2):
+        rows = slice(2 * mb, 2 * mb + 2)
+        h = (ids[rows],)
+        for part in parts:
+            h = part(*h, lengths=lengths[rows])
+            h = h if isinstance(h, tuple) else (h,)
+        want.append(causal_lm_loss(h[0], target[rows]))
+    # the losses are fp32 sums of 64 exponentials and some 30 tokens, the same on both sides but for their place in a batch
+    assert abs(loss - torch.stack(want).mean()) < 100 * 2.0 ** -24 * loss, (loss, want, pipe.losses)
+
+
+@pytest.mark.parametrize("schedule", ["1f1b", "interleaved_1f1b", "zero_bubble"])
+def test_lengths_through_a_pipeline(schedule):
+    run_ranks(_train, 2, schedule)
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+def test_operators_together_on_the_gpu():
+    """A GPT-2 with scaled embeddings, packed documents, sorted table gradients and dropout: the same in bf16 on the GPU, in the
+    kernels, as on the CPU in 64 bits, whose masks are the same; and the same bits again."""
+    from pippy_b200.models.gpt2 import GPT2Config, GPT2Stage
+    from pippy_b200.ops import _lib
+    from pippy_b200.ops import functional as pf
+
+    lengths = torch.tensor([[100, 0, 257, 3], [128, 129, 1, 0], [384, 0, 0, 0]], dtype=torch.int32)
+    S2 = 400
+    cfg = GPT2Config(vocab_size=500, n_positions=S2, dim=128, n_layers=2, n_heads=2, dropout=0.1, sorted_embedding_grad=True)
+    torch.manual_seed(0)
+    model = GPT2Stage(cfg, range(2), True, True, dtype=torch.bfloat16)
+    ids = torch.randint(0, 500, (3, S2))
+    exact = GPT2Stage(cfg, range(2), True, True, dtype=torch.float64)
+    exact.load_state_dict(model.state_dict())
+    model = model.cuda()
+    layout = pf.packed_layout(lengths, S2)
+    inside = (layout.positions >= 0).view(3, S2)
+    g = torch.randn(3, S2, cfg.padded_vocab).bfloat16() * inside.unsqueeze(2)
+
+    def run(m, device, seed):
+        m.zero_grad()
+        for p in m.parameters():
+            p.grad = None
+        draw = pf_draw(seed)
+        old, layers.Dropout.draw = layers.Dropout.draw, staticmethod(lambda d: draw.to(d))
+        try:
+            out = m(ids.to(device), lengths=lengths.to(device))
+            out.backward(g.to(device).to(out.dtype))
+        finally:
+            layers.Dropout.draw = old
+        return out.detach(), {n: p.grad for n, p in m.named_parameters()}
+
+    from pippy_b200.models import layers
+
+    def pf_draw(seed):
+        return torch.tensor([seed])
+
+    out, grads = run(model, "cuda", 7)
+    again, grads2 = run(model, "cuda", 7)
+    assert torch.equal(out, again) and torch.equal(grads["wte.positions"], grads2["wte.positions"])
+    other, _ = run(model, "cuda", 8)
+    assert not torch.equal(out, other)
+    want, wanted = run(exact, "cpu", 7)
+    # about 12 roundings to bf16 a block and 4 around the blocks, each 2^-9 of the value in the mean square, in random directions:
+    # sqrt(28) 2^-9 = 0.010 forward; a gradient passes as many again: sqrt(56) 2^-9 = 0.015.  Twice that.
+    def off(a, b):
+        return ((a.double().cpu() - b).norm() / b.norm()).item()
+
+    assert off(out[inside.cuda()], want[inside]) < 0.02
+    for name, b in wanted.items():
+        assert off(grads[name], b) < 0.03, name
+    _lib.check_device_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpointing", [False, True])
+def test_packed_llama_training_step_on_the_gpu(checkpointing):
+    """A packed batch through a pipeline with fp32 gradient buffers: each gradient against the documents' own, one by one."""
+    from pippy_b200.models.llama import LlamaConfig
+    from pippy_b200.ops import _lib
+    from pippy_b200.train import build_llama_pipeline
+
+    cfg = LlamaConfig.tiny(vocab_size=512, dim=256, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=512)
+    lengths = torch.tensor([[100, 0, 257, 3], [128, 129, 1, 0]], dtype=torch.int32)
+    S2 = 400
+    ids = torch.randint(0, 512, (2, S2), generator=torch.Generator().manual_seed(1))
+    inside = torch.tensor([[t < int(row.sum()) for t in range(S2)] for row in lengths])
+    target = torch.where(inside, ids.roll(-1, 1), -100)
+
+    def build(batch, seq):
+        return build_llama_pipeline(cfg, batch, seq, 1, torch.device("cuda"), schedule="1f1b", lr=0.0, weight_decay=0.0,
+                                    activation_checkpointing=checkpointing)
+
+    pipe = build(2, S2)
+    pipe.optimizer, kept = None, pipe.optimizer
+    pipe.flat.zero_grad()
+    loss = pipe.train_step(ids.cuda(), target.cuda(), lengths.cuda())
+    got = pipe.flat.grad.clone()
+    model = pipe.stages[0].submod
+    pipe.flat.zero_grad()
+    # the same documents, one at a time, each loss weighted as in the packed mean
+    from pippy_b200.models.llama import causal_lm_loss
+
+    total, count = 0.0, int((target != -100).sum())
+    for row in range(2):
+        at = 0
+        for n in lengths[row].tolist():
+            if n:
+                part = causal_lm_loss(model(ids[row : row + 1, at : at + n].cuda()), target[row : row + 1, at : at + n].cuda())
+                (part * (n / count)).backward()
+                total += part.item() * n / count
+            at += n
+    want = pipe.flat.grad.clone()
+    # both sides round the same values to bf16, in tiles of other shapes: sqrt(2) times the 0.015 of the test above, twice
+    assert abs(loss.item() - total) < 0.01 * total
+    assert ((got - want).norm() / want.norm()).item() < 0.04
+    _lib.check_device_errors()
