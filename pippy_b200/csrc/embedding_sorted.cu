@@ -66,6 +66,8 @@ struct Table {
   int2* sorted;  // [T] (key, t), by key and then by t
   int2* other;   // [T] the passes' second buffer
   float* partial;      // [2 * tiles, H]: sums of the runs that enter and that leave a tile
+  int* crossing;       // tiles in which a run begins that leaves them
+  int* n_crossing;     // how many
   void* grad;          // [size, H]: fp32, added to, or bf16, written whole
   float scale;
 };
@@ -180,9 +182,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   __shared__ uint32_t s_total[256], s_base[256], s_scan[8];
   const int cluster = blockIdx.x / kCluster;
   if (cluster < a.tables) {
+    if (blockIdx.x % kCluster == 0 && threadIdx.x == 0) *(cluster == 0 ? a.table[0] : a.table[1]).n_crossing = 0;
     sort_table(a, cluster == 0 ? a.table[0] : a.table[1], s_hist, s_total, s_base, s_scan);
     return;
   }
+  // the other blocks clear; writes alone run at 3.7 TB/s here, with plain stores and with bulk copies alike
   const long long at = (blockIdx.x - a.tables * kCluster) * (long long)blockDim.x + threadIdx.x;
   const long long step = (long long)(gridDim.x - a.tables * kCluster) * blockDim.x;
   for (int k = 0; k < a.tables; ++k) {
@@ -225,6 +229,12 @@ __global__ void __launch_bounds__(128) embed_runs_kernel(SortArgs a, const __nv_
     if (i >= 1 && i <= n) s_tok[i - 1] = e.y;
   }
   __syncthreads();
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    // the last key goes on in the next tile, is one of the table's and did not enter this tile
+    const int key = s_key[n];
+    if (key < tb.size && s_key[n + 1] == key && !(s_key[1] == key && s_key[0] == key))
+      tb.crossing[atomicAdd(tb.n_crossing, 1)] = blockIdx.x;
+  }
   const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (col >= a.H) return;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -266,55 +276,51 @@ __global__ void __launch_bounds__(128) embed_runs_kernel(SortArgs a, const __nv_
   }
 }
 
-// The tile in which a run begins that goes on beyond it adds up the run: its own last partial sum and the first ones of
-// the tiles after it.  Eight warps take consecutive shares of a long run; shares are added in order.
-__global__ void __launch_bounds__(256) embed_fold_kernel(SortArgs a, int tile_rows) {
+// A run that crosses tiles: the last partial sum of the tile that it begins in and the first ones of the tiles after it.
+// kFoldWarps warps take consecutive shares of a long run; shares are added in order.  The list's order is not that of the
+// keys, but each run has a row of its own.  With a third of 32 752 tokens being one id, 1024 columns: 32.7 us when every warp
+// looked for the run's end by itself, 25.0 with the block looking together; 16 warps took 23.5, but 15.3 instead of 10.7 where
+// runs are short (8 192 tokens, 4096 columns).
+constexpr int kFoldWarps = 8;
+
+__global__ void __launch_bounds__(32 * kFoldWarps) embed_fold_kernel(SortArgs a, int tile_rows) {
   const Table& tb = blockIdx.z == 0 ? a.table[0] : a.table[1];
   const long long tiles = (a.T + tile_rows - 1) / tile_rows;
-  const long long tile = blockIdx.x, t0 = tile * tile_rows;
-  const long long next = t0 + tile_rows;
-  if (next >= a.T) return;
-  const int key = tb.sorted[next].x;
-  if (key >= tb.size || tb.sorted[next - 1].x != key) return;                       // no run leaves this tile
-  if (tb.sorted[t0].x == key && t0 > 0 && tb.sorted[t0 - 1].x == key) return;      // it began in an earlier one
+  const int runs = *tb.n_crossing;
   const int lane = threadIdx.x, y = threadIdx.y;
-  long long more = 1;  // tiles after this one that the run reaches
-  for (;;) {
-    const long long t = tile + more + lane;
-    const bool in = t < tiles && tb.sorted[t * tile_rows].x == key;
-    const unsigned got = __ballot_sync(0xffffffffu, in);
-    if (got == 0xffffffffu) {
-      more += 32;
-      continue;
-    }
-    more += __ffs(~got) - 1;
-    break;
-  }
-  more -= 1;  // tile + 1 .. tile + more
   const int col = (blockIdx.y * 32 + lane) * 8;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto add = [&](long long t, int which) {
-    const float4* p = reinterpret_cast<const float4*>(tb.partial + (t * 2 + which) * a.H + col);
-    const float4 lo = p[0], hi = p[1];
-    acc[0] += lo.x, acc[1] += lo.y, acc[2] += lo.z, acc[3] += lo.w;
-    acc[4] += hi.x, acc[5] += hi.y, acc[6] += hi.z, acc[7] += hi.w;
-  };
-  if (col < a.H) {
-    if (y == 0) add(tile, 1);
-    const long long share = (more + 7) / 8;
-    const long long first = tile + 1 + y * share, stop = min(first + share, tile + 1 + more);
-#pragma unroll 4
-    for (long long t = first; t < stop; ++t) add(t, 0);
-  }
-  __shared__ float s_acc[8][32][9];
+  __shared__ float s_acc[kFoldWarps][32][9];
+  for (int r = blockIdx.x; r < runs; r += gridDim.x) {
+    const long long tile = tb.crossing[r];
+    const int key = tb.sorted[(tile + 1) * tile_rows].x;
+    long long more = 0;  // tiles after this one that the run reaches
+    for (int got = 32 * kFoldWarps; got == 32 * kFoldWarps; more += got) {
+      const long long t = tile + 1 + more + y * 32 + lane;
+      got = __syncthreads_count(t < tiles && tb.sorted[t * tile_rows].x == key);
+    }
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto add = [&](long long t, int which) {
+      const float4* p = reinterpret_cast<const float4*>(tb.partial + (t * 2 + which) * a.H + col);
+      const float4 lo = p[0], hi = p[1];
+      acc[0] += lo.x, acc[1] += lo.y, acc[2] += lo.z, acc[3] += lo.w;
+      acc[4] += hi.x, acc[5] += hi.y, acc[6] += hi.z, acc[7] += hi.w;
+    };
+    if (col < a.H) {
+      if (y == 0) add(tile, 1);
+      const long long share = (more + kFoldWarps - 1) / kFoldWarps;
+      const long long first = tile + 1 + y * share, stop = min(first + share, tile + 1 + more);
+#pragma unroll 8
+      for (long long t = first; t < stop; ++t) add(t, 0);
+    }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s_acc[y][lane][j] = acc[j];
-  __syncthreads();
-  if (y == 0 && col < a.H) {
-    for (int k = 1; k < 8; ++k)
+    for (int j = 0; j < 8; ++j) s_acc[y][lane][j] = acc[j];
+    __syncthreads();
+    if (y == 0 && col < a.H) {
+      for (int k = 1; k < kFoldWarps; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += s_acc[k][lane][j];
-    put_row(a, tb, key, col, acc);
+        for (int j = 0; j < 8; ++j) acc[j] += s_acc[k][lane][j];
+      put_row(a, tb, key, col, acc);
+    }
   }
 }
 
@@ -355,7 +361,8 @@ int pb_embed_scaled_fwd(const long long* ids, const void* wte, const void* wpe, 
 long long pb_embed_sorted_scratch(long long T, int H, int tables) {
   using namespace pbs;
   const int rows = tile_rows_for(T, H);
-  return tables * (2 * T * (long long)sizeof(int2) + 2 * ((T + rows - 1) / rows) * H * (long long)sizeof(float) + 32);
+  const long long tiles = (T + rows - 1) / rows;
+  return tables * (2 * T * (long long)sizeof(int2) + 2 * tiles * H * (long long)sizeof(float) + (tiles + 1) * (long long)sizeof(int) + 32);
 }
 
 // dout [T, H] bf16.  gw [vocab, H] and gp [n_positions, H], either null where that gradient is not wanted: fp32 and added to,
@@ -391,7 +398,9 @@ int pb_embed_sorted_bwd(const long long* ids, const int* positions, const void* 
     tb.partial = reinterpret_cast<float*>(at);
     tb.sorted = reinterpret_cast<int2*>(at + 2 * tiles * H * sizeof(float));
     tb.other = tb.sorted + T;
-    at += (2 * tiles * H * sizeof(float) + 2 * T * sizeof(int2) + 15) / 16 * 16;
+    tb.n_crossing = reinterpret_cast<int*>(tb.other + T);
+    tb.crossing = tb.n_crossing + 1;
+    at += (2 * tiles * H * sizeof(float) + 2 * T * sizeof(int2) + (tiles + 1) * sizeof(int) + 15) / 16 * 16;
   }
   const int clearing = write ? 128 : 0;
   embed_sort_kernel<<<a.tables * kCluster + clearing, kSortThreads, 0, stream>>>(a);
@@ -402,7 +411,8 @@ int pb_embed_sorted_bwd(const long long* ids, const int* positions, const void* 
                                                                                  rows);
   pb_count_launch(1);
   if (tiles > 1) {
-    embed_fold_kernel<<<dim3((unsigned)tiles, (H / 8 + 31) / 32, a.tables), dim3(32, 8), 0, stream>>>(a, rows);
+    const long long most = tiles < 148 * 2 ? tiles : 148 * 2;
+    embed_fold_kernel<<<dim3((unsigned)most, (H / 8 + 31) / 32, a.tables), dim3(32, kFoldWarps), 0, stream>>>(a, rows);
     pb_count_launch(1);
   }
   return (int)cudaGetLastError();
