@@ -51,6 +51,22 @@ def test_refusals():
             pf.embedding(torch.tensor([1, 2]), wte, **kw)
 
 
+@pytest.mark.skipif(not _lib.available(), reason="the CUDA library is not built")
+def test_entry_points_refuse_before_they_launch():
+    lib, at = _lib.lib(), 1 << 20  # an address that is only looked at
+
+    def forward(H=64, wpe=None, positions=None, seq=4, out=at):
+        return lib.pb_embed_scaled_fwd(at, at, wpe, positions, out, 8, H, seq, 10, 5, 1.0, at, None)
+
+    def backward(T=8, H=64, V=10, gw=at, gp=None, P=5, seq=4, scratch=at):
+        return lib.pb_embed_sorted_bwd(at, None, at, gw, gp, T, H, seq, V, P, 1.0, 1, scratch, None)
+
+    assert forward(H=12) == forward(H=0) == forward(wpe=at, seq=0) == -1 and forward(out=at + 8) == -2
+    assert backward(H=4) == backward(V=0) == backward(gp=at, P=0) == backward(gp=at, seq=0) == -1
+    assert backward(T=-1) == backward(T=2 ** 31) == backward(V=2 ** 31 - 1) == -2 and backward(scratch=at + 4) == -3
+    assert backward(gw=None) == 0  # no gradient wanted: nothing to do
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 CASES = {  # tokens, rows of the table, width, share of one id
     "one": (1, 5, 8, 0.0),

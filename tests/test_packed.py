@@ -153,6 +153,34 @@ def test_refusals():
         pf.packed_layout(torch.zeros(0, 3, dtype=torch.int32), 4)
 
 
+@pytest.mark.skipif(not _lib.available(), reason="the CUDA library is not built")
+def test_entry_points_refuse_before_they_launch():
+    """Arguments that no launch could take come back as a negative code; nothing here has a GPU to launch on."""
+    lib, at = _lib.lib(), 1 << 20  # an address that is only looked at
+
+    def forward(T=256, Hq=4, Hkv=2, D=64, pitch=512, o=at, tiles=3):
+        return lib.pb_packed_attention_fwd(at, at, at, o, at, at, at, tiles, T, Hq, Hkv, D, pitch, pitch, pitch, 256, 0.1, 1, at, None)
+
+    assert forward(D=32) == forward(D=96) == -1
+    assert forward(Hkv=3) == forward(Hq=0) == forward(Hkv=0) == -2
+    assert forward(pitch=513) == forward(o=at + 8) == -3
+    assert forward(T=0) == forward(T=2 ** 31) == forward(tiles=0) == forward(tiles=2 ** 30) == -4
+
+    def backward(T=256, Hq=4, Hkv=2, D=64, pitch=512, dq=at, tiles=3):
+        return lib.pb_packed_attention_bwd(at, at, at, at, at, at, at, dq, at, at, None, None, 0, at, at, tiles, at, T, Hq, Hkv, D,
+                                           pitch, pitch, pitch, 256, 256, 512, 0.1, 1, at, None)
+
+    assert backward(D=256) == -1 and backward(Hkv=3) == -2 and backward(pitch=4) == backward(dq=at + 2) == -3
+    assert backward(T=0) == backward(tiles=0) == -4
+    assert lib.pb_packed_layout(at, 0, 1, 1, at, at, at, 1, at, 1, at, at, None) == -1
+    assert lib.pb_packed_layout(at, 2 ** 16, 1, 2 ** 16, at, at, at, 1, at, 1, at, at, None) == -2
+    assert lib.pb_packed_rope(at, 64, at, 64, at, at, at, 1, 1, 24, 1, at, None) == -1
+    assert lib.pb_packed_rope(at, 64, at + 8, 64, at, at, at, 1, 1, 64, 1, at, None) == -2
+    # the split of a key head's query heads: none where there are items enough, all of them where there are few
+    plain, split = (lib.pb_packed_attention_bwd_scratch(4096, 32, 4, 128, tiles) for tiles in (2000, 4))
+    assert plain == 4096 * 32 * 4 and split == plain + 8 * 2 * 4096 * 4 * 128 * 4
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _read_tiles(layout, rows):
     tiles, counts = layout.tiles(rows)
@@ -249,6 +277,23 @@ def test_attention_kernel_many_items(heads, D, errors):
         assert torch.isfinite(a).all() and ((a.double() - b).abs() <= bound).all()
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(got, _run(qkv, do, cos, sin, layout, hq, hk, D)))
+
+
+@gpu
+def test_attention_kernel_on_few_sms(errors):
+    """The grid leaves the reserved SMs out; each of the few blocks walks hundreds of items, to the same bits."""
+    from pippy_b200.ops.gemm import set_sm_reserve
+
+    lengths, S, hq, hk, D = [[30, 200, 70, 300], [5, 0, 128, 129]], 640, 16, 4, 128
+    qkv, do, cos, sin = _inputs(lengths, S, hq, hk, D, True, "cuda")
+    layout = _layout(lengths, S, "cuda")
+    want = _run(qkv, do, cos, sin, layout, hq, hk, D)
+    try:
+        for reserve in (145, 10_000):
+            set_sm_reserve(reserve)
+            assert all(torch.equal(a, b) for a, b in zip(want, _run(qkv, do, cos, sin, layout, hq, hk, D)))
+    finally:
+        set_sm_reserve(0)
 
 
 @gpu
