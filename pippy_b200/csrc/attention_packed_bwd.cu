@@ -140,28 +140,28 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp < 4) {
     give_registers<64>();
     if (warp == 0) {
-    while (ok && publish_next()) {
-      const int hkv = h / G;
-      if (!(ok = warp_wait(stage_empty, (it & 1) ^ 1, abort_flag))) break;
-      if (lane == 0) {
-        mbar_expect_tx(stage_full, 2 * TILE_BYTES);
+      while (ok && publish_next()) {
+        const int hkv = h / G;
+        if (!(ok = warp_wait(stage_empty, (it & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) {
+          mbar_expect_tx(stage_full, 2 * TILE_BYTES);
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-          tma_load_2d(sQ + c * kChunkBytes, &tmQ, stage_full, h * D + c * 64, tile.start + tile.rank * 128);
-          tma_load_2d(sDO + c * kChunkBytes, &tmDO, stage_full, h * D + c * 64, tile.start + tile.rank * 128);
+          for (int c = 0; c < NCH; ++c) {
+            tma_load_2d(sQ + c * kChunkBytes, &tmQ, stage_full, h * D + c * 64, tile.start + tile.rank * 128);
+            tma_load_2d(sDO + c * kChunkBytes, &tmDO, stage_full, h * D + c * 64, tile.start + tile.rank * 128);
+          }
         }
-      }
-      for (int j = 0; j < nblk; ++j, ++n) {
-        const int sk = n % kStagesK, sv = n % kStagesV;
-        if (!(ok = warp_wait(&k_empty[sk], ((n / kStagesK) & 1) ^ 1, abort_flag))) break;
-        if (lane == 0)
-          load_tile<NCH>(sK + sk * TILE_BYTES, &tmK, tile.len - j * 128 < 128 ? &k_raw[sk] : &k_full[sk], hkv * D,
-                         tile.start + j * 128);
-        if (!(ok = warp_wait(&v_empty[sv], ((n / kStagesV) & 1) ^ 1, abort_flag))) break;
-        // dP of a key beyond the document is replaced by the mask: V needs no clearing here
-        if (lane == 0) load_tile<NCH>(sV + sv * TILE_BYTES, &tmV, &v_full[sv], hkv * D, tile.start + j * 128);
-      }
-      ++it;
+        for (int j = 0; j < nblk; ++j, ++n) {
+          const int sk = n % kStagesK, sv = n % kStagesV;
+          if (!(ok = warp_wait(&k_empty[sk], ((n / kStagesK) & 1) ^ 1, abort_flag))) break;
+          if (lane == 0)
+            load_tile<NCH>(sK + sk * TILE_BYTES, &tmK, tile.len - j * 128 < 128 ? &k_raw[sk] : &k_full[sk], hkv * D,
+                           tile.start + j * 128);
+          if (!(ok = warp_wait(&v_empty[sv], ((n / kStagesV) & 1) ^ 1, abort_flag))) break;
+          // dP of a key beyond the document is replaced by the mask: V needs no clearing here
+          if (lane == 0) load_tile<NCH>(sV + sv * TILE_BYTES, &tmV, &v_full[sv], hkv * D, tile.start + j * 128);
+        }
+        ++it;
     }
   } else if (warp == 1) {
     // the whole warp walks the loops; one elected lane, the same every time, issues the MMAs and their commits
@@ -480,25 +480,25 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp < 4) {
     give_registers<72>();
     if (warp == 0) {
-    while (ok && publish_next()) {
-      // rows beyond the document stay in their own accumulator rows, which are not written
-      if (!(ok = warp_wait(k_empty, (it & 1) ^ 1, abort_flag))) break;
-      if (lane == 0) load_tile<NCH>(sK, &tmK, k_full, w.hkv * D, w.start + w.kv_tile * 128);
-      int head = (w.hkv * p.split + w.part) * G, blk = w.first;
-      for (int b = 0; b < w.blocks; ++b, ++n) {
-        const int sq = n % kStagesQ, sd = n % kStagesDO;
-        const bool tail = w.len - blk * 128 < 128;
-        if (!(ok = warp_wait(&q_empty[sq], ((n / kStagesQ) & 1) ^ 1, abort_flag))) break;
-        if (lane == 0) load_tile<NCH>(sQ + sq * TILE_BYTES, &tmQ, tail ? &q_raw[sq] : &q_full[sq], head * D, w.start + blk * 128);
-        if (b == 0) {
-          if (!(ok = warp_wait(v_empty, (it & 1) ^ 1, abort_flag))) break;
-          if (lane == 0) load_tile<NCH>(sV, &tmV, v_full, w.hkv * D, w.start + w.kv_tile * 128);
+      while (ok && publish_next()) {
+        // rows beyond the document stay in their own accumulator rows, which are not written
+        if (!(ok = warp_wait(k_empty, (it & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) load_tile<NCH>(sK, &tmK, k_full, w.hkv * D, w.start + w.kv_tile * 128);
+        int head = (w.hkv * p.split + w.part) * G, blk = w.first;
+        for (int b = 0; b < w.blocks; ++b, ++n) {
+          const int sq = n % kStagesQ, sd = n % kStagesDO;
+          const bool tail = w.len - blk * 128 < 128;
+          if (!(ok = warp_wait(&q_empty[sq], ((n / kStagesQ) & 1) ^ 1, abort_flag))) break;
+          if (lane == 0) load_tile<NCH>(sQ + sq * TILE_BYTES, &tmQ, tail ? &q_raw[sq] : &q_full[sq], head * D, w.start + blk * 128);
+          if (b == 0) {
+            if (!(ok = warp_wait(v_empty, (it & 1) ^ 1, abort_flag))) break;
+            if (lane == 0) load_tile<NCH>(sV, &tmV, v_full, w.hkv * D, w.start + w.kv_tile * 128);
+          }
+          if (!(ok = warp_wait(&do_empty[sd], ((n / kStagesDO) & 1) ^ 1, abort_flag))) break;
+          if (lane == 0) load_tile<NCH>(sDO + sd * TILE_BYTES, &tmDO, tail ? &do_raw[sd] : &do_full[sd], head * D, w.start + blk * 128);
+          if (++blk == w.tiles) blk = w.first, ++head;
         }
-        if (!(ok = warp_wait(&do_empty[sd], ((n / kStagesDO) & 1) ^ 1, abort_flag))) break;
-        if (lane == 0) load_tile<NCH>(sDO + sd * TILE_BYTES, &tmDO, tail ? &do_raw[sd] : &do_full[sd], head * D, w.start + blk * 128);
-        if (++blk == w.tiles) blk = w.first, ++head;
-      }
-      ++it;
+        ++it;
     }
   } else if (warp == 1) {
     const uint32_t idesc_t = make_idesc_bf16(128, 128, 0, 0);
@@ -828,7 +828,7 @@ int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const 
   for (const void* x : {o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)cs, (const void*)sn, (const void*)scratch})
     all |= reinterpret_cast<uintptr_t>(x);
   if (all & 15) return -3;
-  if (T < 1 || T > 0x7fffffffLL || max_tiles < 1 || (long long)max_tiles * Hq > 0x7fffffffLL) return -4;
+  if (T < 1 || T > 0x3fffffffLL || max_tiles < 1 || (long long)max_tiles * Hq > 0x7fff0000LL) return -4;  // room for Items' last turn
   CUtensorMap tq, tk, tv, tdo;
   int r = 0;
   r |= pb::make_tmap_bf16_2d(&tq, q, (uint64_t)Hq * D, T, (uint64_t)q_stride, 64, 128);

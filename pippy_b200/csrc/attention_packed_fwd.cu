@@ -157,27 +157,27 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp < 4) {
     give_registers<88>();
     if (warp == 0) {
-    while (ok && publish_next()) {
-      if (w.blocks[0] == 0) continue;
+      while (ok && publish_next()) {
+        if (w.blocks[0] == 0) continue;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (w.blocks[t] == 0 || !ok) continue;
-        ok = warp_wait(&q_empty[t], (used[t] & 1) ^ 1, abort_flag);
-        if (ok && lane == 0) load_tile<NCH>(sQ + t * TILE_BYTES, &tmQ, &q_full[t], w.head[t] * D, w.start + w.row[t]);
-        ++used[t];
-      }
-      const int stages = w.split ? 2 : max(w.blocks[0], w.blocks[1]);
-      for (int j = 0; ok && j < stages; ++j, ++n) {
-        const int s = n & 1;
-        const uint32_t ph = ((n >> 1) & 1) ^ 1;
-        const int col = (w.head[w.split ? j : 0] / G) * D, key = w.split ? 0 : j * 128;
-        if (!(ok = warp_wait(&k_empty[s], ph, abort_flag))) break;
-        // keys beyond the document only make scores that the mask replaces: K needs no clearing, V does
-        if (lane == 0) load_tile<NCH>(sK + s * TILE_BYTES, &tmK, &k_full[s], col, w.start + key);
-        if (!(ok = warp_wait(&v_empty[s], ph, abort_flag))) break;
-        if (lane == 0)
-          load_tile<NCH>(sV + s * TILE_BYTES, &tmV, w.len - key < 128 ? &v_raw[s] : &v_full[s], col, w.start + key);
-      }
+        for (int t = 0; t < 2; ++t) {
+          if (w.blocks[t] == 0 || !ok) continue;
+          ok = warp_wait(&q_empty[t], (used[t] & 1) ^ 1, abort_flag);
+          if (ok && lane == 0) load_tile<NCH>(sQ + t * TILE_BYTES, &tmQ, &q_full[t], w.head[t] * D, w.start + w.row[t]);
+          ++used[t];
+        }
+        const int stages = w.split ? 2 : max(w.blocks[0], w.blocks[1]);
+        for (int j = 0; ok && j < stages; ++j, ++n) {
+          const int s = n & 1;
+          const uint32_t ph = ((n >> 1) & 1) ^ 1;
+          const int col = (w.head[w.split ? j : 0] / G) * D, key = w.split ? 0 : j * 128;
+          if (!(ok = warp_wait(&k_empty[s], ph, abort_flag))) break;
+          // keys beyond the document only make scores that the mask replaces: K needs no clearing, V does
+          if (lane == 0) load_tile<NCH>(sK + s * TILE_BYTES, &tmK, &k_full[s], col, w.start + key);
+          if (!(ok = warp_wait(&v_empty[s], ph, abort_flag))) break;
+          if (lane == 0)
+            load_tile<NCH>(sV + s * TILE_BYTES, &tmV, w.len - key < 128 ? &v_raw[s] : &v_full[s], col, w.start + key);
+        }
     }
   } else if (warp == 1) {
     // the whole warp walks the loops; one elected lane, the same every time, issues the MMAs and their commits
@@ -363,7 +363,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const float2 lb = both(l2);
       const float l = lb.x + lb.y, inv_l = 1.f / l;
       // through memory of the warp's own, 128-byte pieces of 32 rows at a time: whole lines leave (see write_rows in
-      // attention_packed_bwd.cu)
+      // attention_packed_bwd.cuh)
       const int first = first_row + quarter * 32;
       __nv_bfloat16* dst = p.o + ((long long)w.start + first) * p.o_stride + h * D;
       uint8_t* stage = sOut + (warp - 4) * 4096;
@@ -426,7 +426,7 @@ int pb_packed_attention_fwd(const void* q, const void* k, const void* v, void* o
   if (Hq < 1 || Hkv < 1 || Hq % Hkv != 0) return -2;
   if ((q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (o_stride % 8)) return -3;
   if (reinterpret_cast<uintptr_t>(o) & 15) return -3;
-  if (T < 1 || T > 0x7fffffffLL || max_tiles < 1 || (long long)max_tiles * Hq > 0x7fffffffLL) return -4;
+  if (T < 1 || T > 0x3fffffffLL || max_tiles < 1 || (long long)max_tiles * Hq > 0x7fff0000LL) return -4;  // room for Items' last turn
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   CUtensorMap tq, tk, tv;
   if (pb::make_tmap_bf16_2d(&tq, q, (uint64_t)Hq * D, T, (uint64_t)q_stride, 64, 128)) return -10;

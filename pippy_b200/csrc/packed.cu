@@ -218,7 +218,8 @@ int pb_packed_layout(const int* lengths, int rows, int docs, int seq, int* posit
   using namespace pbk;
   if (rows < 1 || docs < 0 || seq < 1) return -1;
   const long long blocks = 1 + (long long)rows * ((seq + kChunk - 1) / kChunk);
-  if ((long long)rows * seq > 0x7fffffffLL || (long long)rows * (docs + 1) > 0x7fffffffLL || blocks > 0x7fffffffLL) return -2;
+  // half of the range, so that a token's number plus a block's step is one of 32 bits too
+  if ((long long)rows * seq > 0x3fffffffLL || (long long)rows * (docs + 1) > 0x3fffffffLL || blocks > 0x3fffffffLL) return -2;
   LayoutArgs a;
   a.lengths = lengths;
   a.rows = rows, a.docs = docs, a.seq = seq;

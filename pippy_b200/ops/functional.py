@@ -582,9 +582,16 @@ class _EmbeddingFn(torch.autograd.Function):
         return None, None, None, None
 
 
+# What ties the op below to autograd.  Its gradients are written by the kernels, and a table as an input would bring the
+# table's accumulation node along, which belongs to the stream of whichever graph made it: with an eager one alive, a
+# captured backward would wait for that stream.  A leaf on the CPU has no stream.
+_TIE = torch.empty(0, requires_grad=True)
+
+
 class _SortedEmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, wte, wpe, positions, S: int, scale: float):
+    def forward(ctx, tie, ids, tables, positions, S: int, scale: float):
+        wte, wpe = tables
         T, H = ids.numel(), wte.shape[1]
         table, ptable = wte, wpe
         if wte.data_ptr() % 16 or not wte.is_contiguous():
@@ -676,12 +683,19 @@ def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 
         if wte.dim() != 2 or wte.shape[1] % 8 or (wpe is not None and (
                 wpe.shape[1:] != wte.shape[1:] or wpe.dtype != wte.dtype or wpe.device != wte.device)):
             raise ValueError("tables: [rows, H] of one type on one device, H a multiple of 8")
+        if wpe is wte:
+            raise ValueError("one tensor as both tables: their gradients are written at the same time")
+        trained = [w for w in (wte, wpe) if w is not None and w.requires_grad]
+        if not all(w.is_leaf for w in trained):
+            raise ValueError("tables that require gradients have to be leaves: the kernels write their gradients")
         if positions is not None:
             if positions.dtype != torch.int32 or not positions.is_contiguous():
-                positions = positions.to(torch.int32).contiguous()
+                # positions beyond 32 bits would wrap to ones that seem to fit
+                positions = positions.long().clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()
         if ids.dtype != torch.int64 or not ids.is_contiguous():
             ids = ids.long().contiguous()
-        return _SortedEmbeddingFn.apply(ids, wte, wpe, positions, S, float(scale))
+        return _SortedEmbeddingFn.apply(_TIE if trained else None, ids, (wte, wpe), positions,
+                                        S if ids.numel() else 1, float(scale))
     if plain:
         out = F.embedding(ids.reshape(-1), wte)
         if wpe is not None:
@@ -742,8 +756,8 @@ def packed_layout(lengths: torch.Tensor, tokens_per_row: int) -> PackedLayout:
         raise ValueError(f"lengths: integers [rows, documents], got {tuple(lengths.shape)} {lengths.dtype}")
     rows, docs = lengths.shape
     S = int(tokens_per_row)
-    if S < 1 or rows * S >= 2 ** 31 or rows * (docs + 1) >= 2 ** 31:
-        raise ValueError(f"{rows} rows of {S} tokens with {docs} documents each: between 1 and 2^31 - 1 of both")
+    if S < 1 or rows * S >= 2 ** 30 or rows * (docs + 1) >= 2 ** 30:
+        raise ValueError(f"{rows} rows of {S} tokens with {docs} documents each: between 1 and 2^30 - 1 of both")
     if not lengths.is_cuda:
         if docs and (bool((lengths < 0).any()) or int(lengths.long().sum(1).max()) > S):
             raise ValueError(f"document lengths are negative or exceed the row of {S} tokens")
@@ -757,7 +771,7 @@ def packed_layout(lengths: torch.Tensor, tokens_per_row: int) -> PackedLayout:
         return PackedLayout(lengths, S, positions.reshape(-1))
     with _on_device_of(lengths):
         # lengths beyond 32 bits would wrap to ones that seem to fit
-        given = (lengths if lengths.dtype == torch.int32 else lengths.clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
+        given = (lengths if lengths.dtype == torch.int32 else lengths.long().clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
         segments = rows * (docs + 1)
         spare = min(segments, rows * S)
         n128, n256 = rows * S // 128 + spare, rows * S // 256 + spare
@@ -829,8 +843,9 @@ class _PackedAttentionFn(torch.autograd.Function):
                 lib.pb_packed_attention_bwd(
                     do.data_ptr(), q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), scratch.data_ptr(), d, d + 2 * nq,
                     d + 2 * (nq + nk), _lib.addr(cos), _lib.addr(sin), 0 if cos is None else cos.shape[0], t128, counts,
-                    layout._most[0], layout.positions.data_ptr(), T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, nq, nq + 2 * nk, scale, int(causal),
-                    _lib.err_addr(qkv.device), _lib.stream_addr()),
+                    layout._most[0], layout.positions.data_ptr(), T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, nq,
+                    nq + 2 * nk, scale, int(causal), _lib.err_addr(qkv.device),
+                    _lib.stream_addr()),
                 "pb_packed_attention_bwd",
             )
         return dqkv, None, None, None, None, None, None, None, None, None
@@ -872,7 +887,7 @@ def packed_attention(qkv, cos, sin, layout: PackedLayout, Hq: int, Hkv: int, D: 
         if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1] or qkv.data_ptr() % 16:
             if inplace and cos is not None:
                 raise ValueError("inplace needs rows of unit stride that start on 16-byte boundaries")
-            qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
         if cos is not None:
             cos, sin = _aligned(cos), _aligned(sin)
         return _PackedAttentionFn.apply(qkv, cos, sin, layout, Hq, Hkv, D, scale, causal, inplace)

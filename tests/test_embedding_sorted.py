@@ -215,3 +215,42 @@ def test_kernel_streams_graph_and_deferral(errors):
     assert not wte.main_grad.any()
     queue.run()
     assert torch.equal(wte.main_grad, want[0])
+
+
+@gpu
+def test_kernel_captured_while_an_eager_graph_of_the_tables_lives(errors):
+    T, V, H = 300, 50, 64
+    ids, gen = _ids(T, V, 0.2)
+    wte, wpe = (torch.nn.Parameter(torch.randn(n, H, generator=gen).bfloat16().cuda()) for n in (V, 100))
+    dout = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    for p in (wte, wpe):
+        p.main_grad = torch.zeros(p.shape, device="cuda")
+    eager = pf.embedding(ids, wte, wpe, 100, sorted_grad=True)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        pf.embedding(ids, wte, wpe, 100, sorted_grad=True).backward(dout)
+    eager.backward(dout)
+    want = [p.main_grad.clone() for p in (wte, wpe)]
+    for p in (wte, wpe):
+        p.main_grad.zero_()
+    graph.replay()
+    assert all(w.any() and torch.equal(p.main_grad, w) for p, w in zip((wte, wpe), want))
+
+
+@gpu
+def test_kernel_empty_batch_wide_positions_and_refusals(errors):
+    wte, wpe = (torch.nn.Parameter(torch.ones(n, 16, device="cuda").bfloat16()) for n in (60, 7))
+    out = pf.embedding(torch.zeros(2, 0, dtype=torch.long, device="cuda"), wte, wpe, sorted_grad=True)
+    out.backward(torch.ones_like(out))
+    assert out.shape == (0, 16) and not wte.grad.any() and not wpe.grad.any()
+    ids = torch.tensor([1, 2, 3], device="cuda")
+    positions = torch.tensor([2, -5, 2 ** 32 + 1], device="cuda")  # the last would be 1 in 32 bits
+    with torch.no_grad():
+        assert torch.equal(pf.embedding(ids, wte, wpe, positions=positions)[:, 0].float().cpu(), torch.tensor([2.0, 1.0, 1.0]))
+    with pytest.raises(_lib.KernelError, match="code 5"):
+        _lib.check_device_errors()
+    with pytest.raises(ValueError, match="both tables"):
+        pf.embedding(ids, wte, wte, sorted_grad=True)
+    with pytest.raises(ValueError, match="leaves"):
+        pf.embedding(ids, wte * 2, sorted_grad=True)

@@ -218,6 +218,14 @@ def test_layout_kernel(case, errors):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int64])
+def test_layout_kernel_takes_every_integer_type(dtype, errors):
+    lengths = [[100, 0, 7], [120, 3, 1]]
+    layout = pf.packed_layout(torch.tensor(lengths, dtype=dtype, device="cuda"), 130)
+    assert torch.equal(layout.positions.cpu(), _positions(lengths, 130))
+
+
+@gpu
 @pytest.mark.parametrize("lengths", [[[5, -1, 4]], [[5, 9, 3]], [[2 ** 31 - 1, 2 ** 31 - 1, 3]], [[2 ** 40, 1, 1]]])
 def test_layout_kernel_cuts_bad_lengths(lengths):
     """Nothing reaches beyond its row: the tiles and positions are those of the lengths cut to what fits, and the host hears of it."""
@@ -361,6 +369,17 @@ def test_attention_kernel_strides_and_inplace(errors):
         pf.packed_attention(torch.zeros(S, 8 * 32, device="cuda").bfloat16(), None, None, layout, 4, 2, 32)
     with pytest.raises(ValueError):
         pf.packed_attention(qkv, cos, sin, _layout(lengths, S, "cpu"), hq, hk, D)
+
+
+@gpu
+def test_attention_kernel_one_row_of_odd_pitch(errors):
+    """A dimension of one row may have any stride."""
+    hq, hk, D = 2, 1, 64
+    qkv, do, cos, sin = _inputs([[1]], 1, hq, hk, D, True, "cuda")
+    want = _run(qkv, do, cos, sin, _layout([[1]], 1, "cuda"), hq, hk, D)
+    odd = qkv.clone().as_strided(qkv.shape, (5, 1))
+    got = _run(odd, do, cos, sin, _layout([[1]], 1, "cuda"), hq, hk, D)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @gpu
