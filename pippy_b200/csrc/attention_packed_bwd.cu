@@ -74,6 +74,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  let_next_start();
   const int count = p.counts[1];  // longer documents only: see attention_packed_short.cu
   const int G = p.Hq / p.Hkv;
   // an item: a tile of queries of head h and the blocks of keys that it sees
@@ -349,6 +350,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
   }
   if (!ok && lane == 0) atomicExch(p.err, ERR_WAIT_TIMEOUT);
+  // its memory and that of the launch before are apart; what follows may need both
+  if (threadIdx.x == 0) after_previous();
   leave(abort_flag, warp, tmem_base);
 }
 
@@ -401,6 +404,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  after_previous();
+  let_next_start();
   const int count = p.counts[1];  // longer documents only: see attention_packed_short.cu
   const int G = p.Hq / p.Hkv / p.split;  // query heads of an item
   // an item: rows [k0, k0 + 128) of a document as keys, blocks [first, tiles) of queries of G heads.  The table lists tiles by
@@ -725,6 +730,7 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(BwdArgs p, const in
   constexpr int kPer = D / 8;
   const int width = p.Hkv * D, per_row = p.Hkv * kPer;
   const long long size = p.T * width;
+  after_previous();
   for (long long t = blockIdx.x * (long long)blockDim.y + threadIdx.y; t < p.T; t += (long long)gridDim.x * blockDim.y) {
     const int pos = positions[t];
     for (int i = threadIdx.x; i < per_row; i += blockDim.x) {
@@ -782,23 +788,30 @@ static int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   constexpr auto pass2 = packed_dkv_kernel<D, kTurn>;
   if (cudaError_t e = pb::allow_smem<pass1, SMEM1>(); e != cudaSuccess) return (int)e;
   if (cudaError_t e = pb::allow_smem<pass2, SMEM2>(); e != cudaSuccess) return (int)e;
+  // The short documents first: their launch needs nothing from the others, and so the blocks of pass 1 take the places that its
+  // last blocks leave.
+  if (int rc = launch_short_bwd<D, kTurn>(tq, tdo, tk, tv, p, dq, dk, dv, stream)) return rc;
   p.out_a = dq;
   p.head_group = attention_head_group(p.max_tiles, p.Hq);
-  pass1<<<resident_blocks((long long)p.max_tiles * p.Hq), kDqThreads, SMEM1, stream>>>(tq, tdo, tk, tv, p);
-  pb_count_launch(1);
+  pb_count_launch(2);
+  if (cudaError_t e = launch_chained(pass1, resident_blocks((long long)p.max_tiles * p.Hq), kDqThreads, SMEM1, stream, tq, tdo, tk, tv, p);
+      e != cudaSuccess)
+    return (int)e;
   p.out_a = dk;
   p.out_b = dv;
   p.head_group = attention_head_group(p.max_tiles, p.Hkv * p.split);
-  pass2<<<resident_blocks((long long)p.max_tiles * p.Hkv * p.split), kDkvThreads, SMEM2, stream>>>(tq, tdo, tk, tv, p);
-  pb_count_launch(1);
-  if (int rc = launch_short_bwd<D, kTurn>(tq, tdo, tk, tv, p, dq, dk, dv, stream)) return rc;
+  if (cudaError_t e = launch_chained(pass2, resident_blocks((long long)p.max_tiles * p.Hkv * p.split), kDkvThreads, SMEM2, stream, tq, tdo,
+                                     tk, tv, p);
+      e != cudaSuccess)
+    return (int)e;
   if (p.split > 1) {
     const int x = p.Hkv * D / 8 < 256 ? (p.Hkv * D / 8 + 31) / 32 * 32 : 256, y = 256 / x;
     const long long blocks = (p.T + y - 1) / y;
-    packed_dkv_sum_kernel<D><<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), dim3(x, y), 0, stream>>>(p, positions);
     pb_count_launch(1);
+    return (int)launch_chained(packed_dkv_sum_kernel<D>, (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), dim3(x, y), 0, stream, p,
+                               positions);
   }
-  return (int)cudaGetLastError();
+  return 0;
 }
 
 }  // namespace pbv

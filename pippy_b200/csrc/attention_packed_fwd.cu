@@ -67,6 +67,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  after_previous();
+  let_next_start();
   const int n_all = p.counts[0], n_wide = p.counts[1], n_docs = p.counts[2];
   const int G = p.Hq / p.Hkv, head_pairs = (p.Hq + 1) / 2;
 
@@ -405,9 +407,8 @@ static int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   constexpr int SMEM = 6 * (D / 64) * kChunkBytes + 32768 + 256 + ItemRing::kBytes;
   constexpr auto kern = packed_fwd_kernel<D>;
   if (cudaError_t e = pb::allow_smem<kern, SMEM>(); e != cudaSuccess) return (int)e;
-  kern<<<resident_blocks((long long)max_tiles * p.Hq), kFwdThreads, SMEM, stream>>>(tq, tk, tv, p);
   pb_count_launch(1);
-  return (int)cudaGetLastError();
+  return (int)pb::launch_chained(kern, resident_blocks((long long)max_tiles * p.Hq), kFwdThreads, SMEM, stream, tq, tk, tv, p);
 }
 
 }  // namespace pbv

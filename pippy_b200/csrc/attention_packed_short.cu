@@ -69,6 +69,7 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int G = p.Hq / p.Hkv / p.split;  // query heads of an item
+  let_next_start();
   const int first_entry = p.counts[1], n_all = p.counts[0] - first_entry;
   const int heads = p.Hkv * p.split;
 

@@ -23,4 +23,25 @@ cudaError_t allow_smem() {
   return e;
 }
 
+// A launch whose blocks may take their places as the blocks of the launch before them leave, once all of these have called
+// let_next_start().  Such a kernel calls after_previous() before it touches memory that earlier launches wrote or read
+// (or, where its own memory and the one before it are apart, before it ends: a launch counts as complete without it).
+template <class... P, class... A>
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+#ifdef __CUDACC__
+// Waits until the launches that this one was chained to are complete and their writes visible.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Called by every block, after after_previous() at the earliest, so that no launch runs ahead of the one before the last.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+
 }  // namespace pb

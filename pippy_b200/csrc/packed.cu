@@ -1,5 +1,6 @@
 // Documents of different lengths packed into rows of equal length: the layout (positions and tile tables, from the lengths
 // alone, on the device) and rotary embedding by position.
+#include "launch.cuh"
 #include "packed.cuh"
 
 #include <cuda_bf16.h>
@@ -137,6 +138,7 @@ __device__ void plan_tiles(const LayoutArgs& a, int* s_hist, int* s_part) {
 __global__ void __launch_bounds__(kPlanThreads) layout_kernel(LayoutArgs a) {
   __shared__ int s_hist[2 * kCounters];
   __shared__ int s_part[kPlanThreads / 32];
+  pb::let_next_start();
   if (blockIdx.x == 0) {
     plan_tiles(a, s_hist, s_part);
     return;
@@ -171,6 +173,8 @@ __global__ void __launch_bounds__(256) packed_rope_kernel(const __nv_bfloat16* s
                                                           const int* __restrict__ positions, long long T, int heads,
                                                           int half, int table_rows, int* err) {
   const int per_head = half / 8, n = heads * per_head;
+  pb::after_previous();
+  pb::let_next_start();
   for (long long t = blockIdx.x; t < T; t += gridDim.x) {
     int pos = positions[t];
     if (pos >= table_rows) {
@@ -244,11 +248,10 @@ int pb_packed_rope(const void* src, long long src_stride, void* dst, long long d
     return -2;
   if (T == 0) return 0;
   const unsigned grid = (unsigned)(T < 148 * 16 ? T : 148 * 16);
-  packed_rope_kernel<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream_)>>>(
-      reinterpret_cast<const __nv_bfloat16*>(src), src_stride, reinterpret_cast<__nv_bfloat16*>(dst), dst_stride, cs, sn,
-      positions, T, heads, D / 2, table_rows, err_dev);
   pb_count_launch(1);
-  return (int)cudaGetLastError();
+  return (int)pb::launch_chained(packed_rope_kernel, grid, 256, 0, reinterpret_cast<cudaStream_t>(stream_),
+                                 reinterpret_cast<const __nv_bfloat16*>(src), src_stride, reinterpret_cast<__nv_bfloat16*>(dst),
+                                 dst_stride, cs, sn, positions, T, heads, D / 2, table_rows, err_dev);
 }
 
 }  // extern "C"
