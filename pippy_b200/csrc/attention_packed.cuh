@@ -111,20 +111,27 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int valid, uint64_t* f
   if (lane == 0) mbar_arrive(full);
 }
 
-// The blocks of a launch stay and take the work items i = 0, 1, ... (tile of the table, head; longest first) in turns, every
-// other turn in reverse, so that no block gets the longer item of every turn.  All roles of a block walk the same sequence.
+// The blocks of a launch stay and take the work items i = 0, 1, ... (tile of the table, head; longest first): from a counter,
+// which begins at 0, whenever they have loaded what the present item needs; without a counter in turns, every other turn
+// in reverse, so that no block gets the longer item of every turn.  The results do not depend on who takes what.  One warp
+// of a block calls next().
 struct Items {
-  int n, turn, i;
-  __device__ __forceinline__ explicit Items(int count) : n(count), turn(-1), i(0) {}
+  int n, turn;
+  int* counter;
+  __device__ __forceinline__ Items(int count, int* counter_) : n(count), turn(-1), counter(counter_) {}
   // next item of this block, -1 after the last
-  __device__ __forceinline__ int next() {
-    for (;;) {
-      ++turn;
+  __device__ __forceinline__ int next(int lane) {
+    ++turn;
+    int i;
+    if (turn == 0 || counter == nullptr) {
       const long long first = (long long)turn * gridDim.x;
       if (first >= n) return -1;
       i = (int)first + ((turn & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
-      if (i < n) return i;
+    } else {
+      i = lane == 0 ? (int)gridDim.x + atomicAdd(counter, 1) : 0;
+      i = __shfl_sync(0xffffffffu, i, 0);
     }
+    return i < n ? i : -1;
   }
 };
 
@@ -191,5 +198,9 @@ inline unsigned resident_blocks(long long items) {
   if (sms < 1) sms = 1;
   return (unsigned)(items < sms ? items : sms);
 }
+
+// Whether a launch takes its items from a counter: not for two turns of them or fewer, which it cannot balance much, and
+// clearing it may take a launch of its own.
+inline bool takes_from_counter(long long items) { return items > 2LL * resident_blocks(items); }
 
 }  // namespace pbv

@@ -75,15 +75,16 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   let_next_start();
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.counter) *p.counter = 0;  // pass 2's
   const int count = p.counts[1];  // longer documents only: see attention_packed_short.cu
   const int G = p.Hq / p.Hkv;
   // an item: a tile of queries of head h and the blocks of keys that it sees
-  Items items(count * p.Hq);
+  Items items(count * p.Hq, nullptr);
   bool ok = true;
   Tile tile;
   int h = 0, nblk = 0;
   auto publish_next = [&]() {  // by the loading warp; false after the last
-    const int i = items.next();
+    const int i = items.next(lane);
     tile.start = -1;
     if (i >= 0) {
       const TileOrder order = tile_order(i, count, p.Hq, p.head_group);
@@ -413,7 +414,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   struct Item {
     int start, len, hkv, part, kv_tile, first, tiles, blocks;
   };
-  Items items(count * p.Hkv * p.split);
+  Items items(count * p.Hkv * p.split, p.counter);
   bool ok = true;
   Item w;
   auto decode = [&](int i) {
@@ -427,7 +428,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     w.blocks = G * (w.tiles - w.first);
   };
   auto publish_next = [&]() {  // by the loading warp; false after the last
-    const int i = items.next();
+    const int i = items.next(lane);
     w.start = -1;
     if (i >= 0) decode(i);
     ok = ring.put(make_int4(w.start, w.len, w.hkv, w.kv_tile), make_int4(w.first, w.tiles, w.blocks, w.part), make_int4(0, 0, 0, 0), lane, abort_flag);
@@ -824,7 +825,7 @@ extern "C" {
 // 128-row tiles; positions: the layout's.
 long long pb_packed_attention_bwd_scratch(long long T, int Hq, int Hkv, int D, int max_tiles) {
   const int split = pbv::split_for(max_tiles, Hq, Hkv);
-  return (T * Hq * 4 + 15) / 16 * 16 + (split > 1 ? split * 2 * T * Hkv * D * 4 : 0);
+  return 16 + (T * Hq * 4 + 15) / 16 * 16 + (split > 1 ? split * 2 * T * Hkv * D * 4 : 0);
 }
 
 int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o,
@@ -854,9 +855,11 @@ int pb_packed_attention_bwd(const void* dO, const void* q, const void* k, const 
   p.o = reinterpret_cast<const __nv_bfloat16*>(o);
   p.o_stride = o_stride;
   p.lse = lse;
-  p.delta = reinterpret_cast<float*>(scratch);
+  p.delta = reinterpret_cast<float*>(scratch) + 4;
   p.split = split_for(max_tiles, Hq, Hkv);
-  p.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(scratch) + (T * Hq * 4 + 15) / 16 * 16);
+  // pass 1 has tiles of about one length in every turn: its items in turns were within 3% of evenly spread in every case here
+  p.counter = takes_from_counter((long long)max_tiles * Hkv * p.split) ? reinterpret_cast<int*>(scratch) : nullptr;
+  p.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(scratch) + 16 + (T * Hq * 4 + 15) / 16 * 16);
   p.out_stride = dqkv_stride;
   p.cs = cs, p.sn = sn;
   p.table_rows = table_rows;

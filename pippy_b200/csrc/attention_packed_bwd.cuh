@@ -23,6 +23,7 @@ struct BwdArgs {
   float scale, scale_log2;
   int causal;
   int head_group;
+  int* counter;  // pass 2: of items, see Items
   int* err;
 };
 

@@ -28,6 +28,7 @@ struct FwdArgs {
   float scale_log2;  // softmax scale * log2(e)
   int causal;
   int head_group;
+  int* counter;  // of items, see Items
   int* err;
 };
 
@@ -80,11 +81,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool split;           // two heads with keys of their own (one block each)
   };
   // decoded by the loading warp, taken from the ring by the others; false after the last
-  Items items(n_wide * p.Hq + (n_docs - n_wide) * head_pairs + (n_all - n_docs) * p.Hq);
+  Items items(n_wide * p.Hq + (n_docs - n_wide) * head_pairs + (n_all - n_docs) * p.Hq, p.counter);
   bool ok = true;
   Item w;
   auto decode = [&]() {
-    int i = items.next(), entry;
+    int i = items.next(lane), entry;
     if (i < 0) {
       w.start = -1;
       return;
@@ -416,10 +417,11 @@ static int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 extern "C" {
 
 // q/k/v: bf16 [T, ...], head h at columns [h * D, (h + 1) * D) of the respective pointer, row pitches in elements.
-// o: [T, o_stride] bf16, every row written (zeros in padding); lse: [Hq, T] fp32, rows of documents written.
+// o: [T, o_stride] bf16, every row written (zeros in padding); lse: [Hq, T] fp32, rows of documents written.  counter: a word of
+// this call alone; `cleared` where an earlier launch (pb_packed_rope's) has set it to 0.
 // tiles / counts: the layout's table of 256-row tiles (max_tiles entries at most).
-int pb_packed_attention_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* tiles,
-                            const int* counts, int max_tiles, long long T, int Hq, int Hkv, int D, long long q_stride,
+int pb_packed_attention_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int* counter, int cleared,
+                            const int* tiles, const int* counts, int max_tiles, long long T, int Hq, int Hkv, int D, long long q_stride,
                             long long k_stride, long long v_stride, long long o_stride, float softmax_scale, int causal,
                             int* err_dev, void* stream_) {
   using namespace pbv;
@@ -446,6 +448,12 @@ int pb_packed_attention_fwd(const void* q, const void* k, const void* v, void* o
   p.scale_log2 = softmax_scale * kLog2e;
   p.causal = causal;
   p.err = err_dev;
+  if (takes_from_counter((long long)max_tiles * Hq)) {
+    p.counter = counter;
+    if (!cleared) {
+      if (cudaError_t e = cudaMemsetAsync(counter, 0, sizeof(int), stream); e != cudaSuccess) return (int)e;
+    }
+  }
   p.head_group = pb::attention_head_group(max_tiles, Hq);
   return D == 128 ? launch_fwd<128>(tq, tk, tv, p, max_tiles, stream)
                   : launch_fwd<64>(tq, tk, tv, p, max_tiles, stream);

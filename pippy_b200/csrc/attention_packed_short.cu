@@ -74,11 +74,11 @@ packed_short_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int heads = p.Hkv * p.split;
 
   // an item: a document (or a tile of padding), a key head, and `part` of its query heads
-  Items items(n_all * heads);
+  Items items(n_all * heads, nullptr);
   bool ok = true;
   int start = 0, len = 0, rank = 0, hkv = 0, part = 0, pad = 0;
   auto publish_next = [&]() {  // by the loading warp; false after the last
-    const int i = items.next();
+    const int i = items.next(lane);
     start = -1;
     if (i >= 0) {
       const int entry = i / heads, index = i - entry * heads;

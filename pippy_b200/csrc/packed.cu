@@ -171,10 +171,11 @@ __global__ void __launch_bounds__(256) packed_rope_kernel(const __nv_bfloat16* s
                                                           __nv_bfloat16* dst, long long dst_stride,
                                                           const float* __restrict__ cs, const float* __restrict__ sn,
                                                           const int* __restrict__ positions, long long T, int heads,
-                                                          int half, int table_rows, int* err) {
+                                                          int half, int table_rows, int* clear, int* err) {
   const int per_head = half / 8, n = heads * per_head;
   pb::after_previous();
   pb::let_next_start();
+  if (clear && blockIdx.x == 0 && threadIdx.x == 0) *clear = 0;
   for (long long t = blockIdx.x; t < T; t += gridDim.x) {
     int pos = positions[t];
     if (pos >= table_rows) {
@@ -238,9 +239,10 @@ int pb_packed_layout(const int* lengths, int rows, int docs, int seq, int* posit
   return (int)cudaGetLastError();
 }
 
+// clear: a word that is set to 0 on the way, may be null.
 int pb_packed_rope(const void* src, long long src_stride, void* dst, long long dst_stride, const float* cs,
-                   const float* sn, const int* positions, long long T, int heads, int D, int table_rows, int* err_dev,
-                   void* stream_) {
+                   const float* sn, const int* positions, long long T, int heads, int D, int table_rows, int* clear,
+                   int* err_dev, void* stream_) {
   using namespace pbk;
   if (D % 16 != 0 || src_stride % 8 != 0 || dst_stride % 8 != 0) return -1;
   if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(cs) |
@@ -251,7 +253,7 @@ int pb_packed_rope(const void* src, long long src_stride, void* dst, long long d
   pb_count_launch(1);
   return (int)pb::launch_chained(packed_rope_kernel, grid, 256, 0, reinterpret_cast<cudaStream_t>(stream_),
                                  reinterpret_cast<const __nv_bfloat16*>(src), src_stride, reinterpret_cast<__nv_bfloat16*>(dst),
-                                 dst_stride, cs, sn, positions, T, heads, D / 2, table_rows, err_dev);
+                                 dst_stride, cs, sn, positions, T, heads, D / 2, table_rows, clear, err_dev);
 }
 
 }  // extern "C"

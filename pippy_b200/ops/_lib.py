@@ -49,9 +49,9 @@ SIGNATURES = {
     "pb_norm_fwd": "p" * 6 + "iifip",
     "pb_packed_attention_bwd": "p" * 12 + "i" "ppip" "liii" "llllll" "fipp",
     "pb_packed_attention_bwd_scratch": "liiii",
-    "pb_packed_attention_fwd": "p" * 7 + "i" "liii" "llll" "fipp",
+    "pb_packed_attention_fwd": "p" * 6 + "i" "ppi" "liii" "llll" "fipp",
     "pb_packed_layout": "piii" "ppp" "ipi" "ppp",
-    "pb_packed_rope": "plpl" "ppp" "liii" "pp",
+    "pb_packed_rope": "plpl" "ppp" "liii" "ppp",
     "pb_rope": "ppp" "liii" "lfp",
     "pb_scale_bf16": "pplp",
     "pb_set_gemm_group_m": "i",

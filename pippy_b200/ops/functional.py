@@ -799,26 +799,27 @@ class _PackedAttentionFn(torch.autograd.Function):
         lib, err = _lib.lib(), _lib.err_addr(qkv.device)
         with _on_device_of(qkv):
             stream = _lib.stream_addr()
+            lse = torch.empty(Hq * T + 1, device=qkv.device, dtype=torch.float32)  # and the forward's counter
+            counter = lse.data_ptr() + 4 * Hq * T
             qk = qkv
             if cos is not None:
                 if not inplace:
                     qk = torch.empty(T, nq + nk, device=qkv.device, dtype=qkv.dtype)
                 _lib.check(
                     lib.pb_packed_rope(qkv.data_ptr(), qkv.stride(0), qk.data_ptr(), qk.stride(0), cos.data_ptr(),
-                                       sin.data_ptr(), layout.positions.data_ptr(), T, Hq + Hkv, D, cos.shape[0], err,
-                                       stream),
+                                       sin.data_ptr(), layout.positions.data_ptr(), T, Hq + Hkv, D, cos.shape[0],
+                                       counter, err, stream),
                     "pb_packed_rope",
                 )
                 if inplace:
                     torch.autograd.graph.increment_version(qkv)
             o = torch.empty(T, nq, device=qkv.device, dtype=qkv.dtype)
-            lse = torch.empty(Hq, T, device=qkv.device, dtype=torch.float32)
             _, t256, _, counts = layout._addresses()
             q, v, pitch = qk.data_ptr(), qkv.data_ptr() + 2 * (nq + nk), qk.stride(0)
             _lib.check(
-                lib.pb_packed_attention_fwd(q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), t256, counts,
-                                            layout._most[1], T, Hq, Hkv, D, pitch, pitch, qkv.stride(0), nq, scale,
-                                            int(causal), err, stream),
+                lib.pb_packed_attention_fwd(q, q + 2 * nq, v, o.data_ptr(), lse.data_ptr(), counter,
+                                            int(cos is not None), t256, counts, layout._most[1], T, Hq, Hkv, D, pitch,
+                                            pitch, qkv.stride(0), nq, scale, int(causal), err, stream),
                 "pb_packed_attention_fwd",
             )
         ctx.save_for_backward(qkv, qk, o, lse, cos, sin)

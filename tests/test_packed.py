@@ -159,7 +159,7 @@ def test_entry_points_refuse_before_they_launch():
     lib, at = _lib.lib(), 1 << 20  # an address that is only looked at
 
     def forward(T=256, Hq=4, Hkv=2, D=64, pitch=512, o=at, tiles=3):
-        return lib.pb_packed_attention_fwd(at, at, at, o, at, at, at, tiles, T, Hq, Hkv, D, pitch, pitch, pitch, 256, 0.1, 1, at, None)
+        return lib.pb_packed_attention_fwd(at, at, at, o, at, at, 1, at, at, tiles, T, Hq, Hkv, D, pitch, pitch, pitch, 256, 0.1, 1, at, None)
 
     assert forward(D=32) == forward(D=96) == -1
     assert forward(Hkv=3) == forward(Hq=0) == forward(Hkv=0) == -2
@@ -174,11 +174,11 @@ def test_entry_points_refuse_before_they_launch():
     assert backward(T=0) == backward(tiles=0) == -4
     assert lib.pb_packed_layout(at, 0, 1, 1, at, at, at, 1, at, 1, at, at, None) == -1
     assert lib.pb_packed_layout(at, 2 ** 16, 1, 2 ** 16, at, at, at, 1, at, 1, at, at, None) == -2
-    assert lib.pb_packed_rope(at, 64, at, 64, at, at, at, 1, 1, 24, 1, at, None) == -1
-    assert lib.pb_packed_rope(at, 64, at + 8, 64, at, at, at, 1, 1, 64, 1, at, None) == -2
+    assert lib.pb_packed_rope(at, 64, at, 64, at, at, at, 1, 1, 24, 1, None, at, None) == -1
+    assert lib.pb_packed_rope(at, 64, at + 8, 64, at, at, at, 1, 1, 64, 1, None, at, None) == -2
     # the split of a key head's query heads: none where there are items enough, all of them where there are few
     plain, split = (lib.pb_packed_attention_bwd_scratch(4096, 32, 4, 128, tiles) for tiles in (2000, 4))
-    assert plain == 4096 * 32 * 4 and split == plain + 8 * 2 * 4096 * 4 * 128 * 4
+    assert plain == 16 + 4096 * 32 * 4 and split == plain + 8 * 2 * 4096 * 4 * 128 * 4
 
 
 # ------------------------------------------------------------------------------------------------ GPU
