@@ -6,6 +6,7 @@
 // The sums are formed in the order of t: the same bits on every run, and a token that fills a third of the batch costs no
 // contended atomics.  Three launches: the tokens are sorted (stable radix sort, one cluster per table), tiles of the sorted
 // order sum their runs of equal tokens, and runs that cross tiles are folded from the tiles' partial sums.
+#include "launch.cuh"
 #include "packed.cuh"
 #include "tc05.cuh"
 
@@ -181,6 +182,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
   __shared__ uint32_t s_hist[kWarps * 256];
   __shared__ uint32_t s_total[256], s_base[256], s_scan[8];
   const int cluster = blockIdx.x / kCluster;
+  pb::let_next_start();
   if (cluster < a.tables) {
     if (blockIdx.x % kCluster == 0 && threadIdx.x == 0) *(cluster == 0 ? a.table[0] : a.table[1]).n_crossing = 0;
     sort_table(a, cluster == 0 ? a.table[0] : a.table[1], s_hist, s_total, s_base, s_scan);
@@ -207,11 +209,11 @@ __device__ __forceinline__ void put_row(const SortArgs& a, const Table& tb, long
     for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(sum[2 * j] * tb.scale, sum[2 * j + 1] * tb.scale);
     *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(tb.grad) + key * a.H + col) = w;
   } else {
+    // An addition that memory makes: the thread need not wait for what is there.  Each element gets one in a launch, so there
+    // is no order that could matter.
     float4* g = reinterpret_cast<float4*>(reinterpret_cast<float*>(tb.grad) + key * a.H + col);
-    float4 lo = g[0], hi = g[1];
-    lo.x += sum[0] * tb.scale, lo.y += sum[1] * tb.scale, lo.z += sum[2] * tb.scale, lo.w += sum[3] * tb.scale;
-    hi.x += sum[4] * tb.scale, hi.y += sum[5] * tb.scale, hi.z += sum[6] * tb.scale, hi.w += sum[7] * tb.scale;
-    g[0] = lo, g[1] = hi;
+    atomicAdd(g, make_float4(sum[0] * tb.scale, sum[1] * tb.scale, sum[2] * tb.scale, sum[3] * tb.scale));
+    atomicAdd(g + 1, make_float4(sum[4] * tb.scale, sum[5] * tb.scale, sum[6] * tb.scale, sum[7] * tb.scale));
   }
 }
 
@@ -222,6 +224,8 @@ __global__ void __launch_bounds__(128) embed_runs_kernel(SortArgs a, const __nv_
   __shared__ int s_key[kMaxTile + 2], s_tok[kMaxTile];
   const long long t0 = (long long)blockIdx.x * tile_rows;
   const int n = (int)(a.T - t0 < tile_rows ? a.T - t0 : tile_rows);
+  pb::after_previous();
+  pb::let_next_start();
   for (int i = threadIdx.x; i < n + 2; i += blockDim.x) {  // one neighbour on each side
     const long long t = t0 - 1 + i;
     const int2 e = t >= 0 && t < a.T ? tb.sorted[t] : make_int2(-1, 0);
@@ -276,51 +280,79 @@ __global__ void __launch_bounds__(128) embed_runs_kernel(SortArgs a, const __nv_
   }
 }
 
-// A run that crosses tiles: the last partial sum of the tile that it begins in and the first ones of the tiles after it.
-// kFoldWarps warps take consecutive shares of a long run; shares are added in order.  The list's order is not that of the
-// keys, but each run has a row of its own.  With a third of 32 752 tokens being one id, 1024 columns: 32.7 us when every warp
-// looked for the run's end by itself, 25.0 with the block looking together; 16 warps took 23.5, but 15.3 instead of 10.7 where
-// runs are short (8 192 tokens, 4096 columns).
+// A run that crosses tiles: the last partial sum of the tile that it begins in and the first ones of the tiles after it, in
+// order.  The list's order is not that of the keys, but each run has a row of its own.  A warp takes a run that ends within 32
+// tiles; a longer one is left to the block, whose warps look for its end together and take consecutive shares.
 constexpr int kFoldWarps = 8;
 
 __global__ void __launch_bounds__(32 * kFoldWarps) embed_fold_kernel(SortArgs a, int tile_rows) {
   const Table& tb = blockIdx.z == 0 ? a.table[0] : a.table[1];
   const long long tiles = (a.T + tile_rows - 1) / tile_rows;
-  const int runs = *tb.n_crossing;
   const int lane = threadIdx.x, y = threadIdx.y;
   const int col = (blockIdx.y * 32 + lane) * 8;
   __shared__ float s_acc[kFoldWarps][32][9];
-  for (int r = blockIdx.x; r < runs; r += gridDim.x) {
-    const long long tile = tb.crossing[r];
-    const int key = tb.sorted[(tile + 1) * tile_rows].x;
-    long long more = 0;  // tiles after this one that the run reaches
-    for (int got = 32 * kFoldWarps; got == 32 * kFoldWarps; more += got) {
-      const long long t = tile + 1 + more + y * 32 + lane;
-      got = __syncthreads_count(t < tiles && tb.sorted[t * tile_rows].x == key);
-    }
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    auto add = [&](long long t, int which) {
-      const float4* p = reinterpret_cast<const float4*>(tb.partial + (t * 2 + which) * a.H + col);
-      const float4 lo = p[0], hi = p[1];
-      acc[0] += lo.x, acc[1] += lo.y, acc[2] += lo.z, acc[3] += lo.w;
-      acc[4] += hi.x, acc[5] += hi.y, acc[6] += hi.z, acc[7] += hi.w;
-    };
-    if (col < a.H) {
-      if (y == 0) add(tile, 1);
-      const long long share = (more + kFoldWarps - 1) / kFoldWarps;
-      const long long first = tile + 1 + y * share, stop = min(first + share, tile + 1 + more);
-#pragma unroll 8
-      for (long long t = first; t < stop; ++t) add(t, 0);
-    }
+  __shared__ int s_long[kFoldWarps];
+  pb::after_previous();
+  const int runs = *tb.n_crossing;
+  float acc[8];
+  auto clear = [&]() {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s_acc[y][lane][j] = acc[j];
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  };
+  auto add = [&](long long t, int which) {
+    const float4* p = reinterpret_cast<const float4*>(tb.partial + (t * 2 + which) * a.H + col);
+    const float4 lo = p[0], hi = p[1];
+    acc[0] += lo.x, acc[1] += lo.y, acc[2] += lo.z, acc[3] += lo.w;
+    acc[4] += hi.x, acc[5] += hi.y, acc[6] += hi.z, acc[7] += hi.w;
+  };
+  for (int r0 = blockIdx.x * kFoldWarps; r0 < runs; r0 += gridDim.x * kFoldWarps) {
+    bool is_long = false;
+    if (r0 + y < runs) {
+      const long long tile = tb.crossing[r0 + y];
+      const long long t = tile + 1 + lane;
+      const int mine = t < tiles ? tb.sorted[t * tile_rows].x : -1, key = __shfl_sync(0xffffffffu, mine, 0);
+      const unsigned same = __ballot_sync(0xffffffffu, mine == key);  // keys are in order: the run's tiles come first
+      is_long = same == 0xffffffffu;
+      if (!is_long && col < a.H) {
+        clear();
+        add(tile, 1);
+        const int more = __popc(same);
+#pragma unroll 4
+        for (int k = 1; k <= more; ++k) add(tile + k, 0);
+        put_row(a, tb, key, col, acc);
+      }
+    }
+    if (lane == 0) s_long[y] = is_long;
     __syncthreads();
-    if (y == 0 && col < a.H) {
-      for (int k = 1; k < kFoldWarps; ++k)
+    for (int w = 0; w < kFoldWarps; ++w) {
+      if (!s_long[w]) continue;
+      const long long tile = tb.crossing[r0 + w];
+      const int key = tb.sorted[(tile + 1) * tile_rows].x;
+      long long more = 0;  // tiles after this one that the run reaches
+      for (int got = 32 * kFoldWarps; got == 32 * kFoldWarps; more += got) {
+        const long long t = tile + 1 + more + y * 32 + lane;
+        got = __syncthreads_count(t < tiles && tb.sorted[t * tile_rows].x == key);
+      }
+      clear();
+      if (col < a.H) {
+        if (y == 0) add(tile, 1);
+        const long long share = (more + kFoldWarps - 1) / kFoldWarps;
+        const long long first = tile + 1 + y * share, stop = min(first + share, tile + 1 + more);
+#pragma unroll 8
+        for (long long t = first; t < stop; ++t) add(t, 0);
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += s_acc[k][lane][j];
-      put_row(a, tb, key, col, acc);
+      for (int j = 0; j < 8; ++j) s_acc[y][lane][j] = acc[j];
+      __syncthreads();
+      if (y == 0 && col < a.H) {
+        for (int k = 1; k < kFoldWarps; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += s_acc[k][lane][j];
+        put_row(a, tb, key, col, acc);
+      }
+      __syncthreads();
     }
+    __syncthreads();  // before s_long is written again
   }
 }
 
@@ -407,13 +439,16 @@ int pb_embed_sorted_bwd(const long long* ids, const int* positions, const void* 
   pb_count_launch(1);
   if (T == 0) return (int)cudaGetLastError();
   const int slabs = (H / 8 + 127) / 128;
-  embed_runs_kernel<<<dim3((unsigned)tiles, slabs, a.tables), 128, 0, stream>>>(a, reinterpret_cast<const __nv_bfloat16*>(dout),
-                                                                                 rows);
   pb_count_launch(1);
+  if (cudaError_t e = pb::launch_chained(embed_runs_kernel, dim3((unsigned)tiles, slabs, a.tables), 128, 0, stream, a,
+                                         reinterpret_cast<const __nv_bfloat16*>(dout), rows);
+      e != cudaSuccess)
+    return (int)e;
   if (tiles > 1) {
-    const long long most = tiles < 148 * 2 ? tiles : 148 * 2;
-    embed_fold_kernel<<<dim3((unsigned)most, (H / 8 + 31) / 32, a.tables), dim3(32, kFoldWarps), 0, stream>>>(a, rows);
+    const long long most = (tiles + kFoldWarps - 1) / kFoldWarps < 148 * 2 ? (tiles + kFoldWarps - 1) / kFoldWarps : 148 * 2;
     pb_count_launch(1);
+    return (int)pb::launch_chained(embed_fold_kernel, dim3((unsigned)most, (H / 8 + 31) / 32, a.tables), dim3(32, kFoldWarps), 0,
+                                   stream, a, rows);
   }
   return (int)cudaGetLastError();
 }
