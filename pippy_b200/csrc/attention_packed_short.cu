@@ -10,6 +10,8 @@
 //     dQ = dS K                              dS read query-major; over dP's columns in TMEM
 // The chain of one head is serial; what overlaps it are the next head's loads and its S.  The
 // products run over the document's tokens, rounded up to 16, and not over the tile.
+// Measured: 190 documents of 59 tokens on average, 32 query and 8 key heads of 128: 208 us, 5.3 us per head of a document and
+// SM.  Bound by that chain: five products of 500 cycles or fewer, two exchanges through shared memory, and the epilogue.
 // Roundings as in the longer documents' kernels.
 // Warps: 0 loads (TMA), 1 issues MMAs and owns TMEM, 2 clears what reaches beyond the document, 4..11 softmax, delta and
 // epilogue (two per TMEM lane quarter, 64 keys each).

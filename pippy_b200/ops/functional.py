@@ -864,7 +864,7 @@ def packed_attention(qkv, cos, sin, layout: PackedLayout, Hq: int, Hkv: int, D: 
     stay unrotated from there on, on the CPU they raise).  With ``inplace`` the rotation overwrites the q and k columns
     of ``qkv`` (its version counter is bumped), which saves a tensor of their size; without rotation it means nothing.
 
-    Kernel path (CUDA bf16): D is 64 or 128, no atomics, the same bits on every run."""
+    Kernel path (CUDA bf16): D is 64 or 128; sums have a fixed order, the same bits on every run."""
     scale = (1.0 / math.sqrt(D)) if scale is None else float(scale)
     if Hq < 1 or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads evenly")

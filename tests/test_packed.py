@@ -418,3 +418,34 @@ def test_attention_kernel_streams_and_graph(errors):
         graph.replay()
         eager = _run(*cases[1 - i][1:], pf.packed_layout(cases[1 - i][0], S), hq, hk, D)
         assert all(torch.equal(a, b) for a, b in zip(out, want[i])) and all(torch.equal(a, b) for a, b in zip(eager, want[1 - i]))
+
+
+@gpu
+@pytest.mark.parametrize("rotary", [True, False])
+def test_attention_kernel_many_items_at_once_and_captured(rotary, errors):
+    """Launches whose blocks take their items from a counter: two calls at once, replays, a backward that runs twice."""
+    lengths, S, hq, hk, D = [[30, 300, 128, 1000, 0, 71], [700, 5, 640, 100, 0, 0]], 1600, 48, 16, 64
+    qkv, do, cos, sin = _inputs(lengths, S, hq, hk, D, rotary, "cuda")
+    layout = _layout(lengths, S, "cuda")
+    want = _run(qkv, do, cos, sin, layout, hq, hk, D)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(_run(qkv, do, cos, sin, layout, hq, hk, D))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for run in got for a, b in zip(run, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _run(qkv, do, cos, sin, layout, hq, hk, D)
+    for _ in range(3):
+        for t in out:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    x = qkv.clone().requires_grad_(True)
+    o = pf.packed_attention(x, cos, sin, layout, hq, hk, D)
+    for _ in range(2):
+        (grad,) = torch.autograd.grad(o, x, do, retain_graph=True)
+        assert torch.equal(grad, want[1])
