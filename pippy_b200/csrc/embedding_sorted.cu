@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(32 * kFoldWarps) embed_fold_kernel(SortArgs a,
         clear();
         add(tile, 1);
         const int more = __popc(same);
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 1; k <= more; ++k) add(tile + k, 0);
         put_row(a, tb, key, col, acc);
       }
