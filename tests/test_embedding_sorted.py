@@ -254,3 +254,20 @@ def test_kernel_empty_batch_wide_positions_and_refusals(errors):
         pf.embedding(ids, wte, wte, sorted_grad=True)
     with pytest.raises(ValueError, match="leaves"):
         pf.embedding(ids, wte * 2, sorted_grad=True)
+
+
+@gpu
+@pytest.mark.parametrize("V,H,T", [(5000, 1024, 40), (5000, 1024, 900), (300, 4096, 64), (129, 2048, 7)])
+def test_kernel_writes_the_rows_that_do_not_occur(V, H, T, errors):
+    """Gradients written whole, with few tokens for the table: zeros in every other row, whatever the memory held."""
+    ids, gen = _ids(T, V, 0.1)
+    ids[0], ids[-1] = 0, V - 1
+    wte, wpe = (torch.nn.Parameter(torch.randn(n, H, generator=gen).bfloat16().cuda()) for n in (V, V + 1))
+    pos = torch.randint(-1, V + 1, (T,), generator=gen).cuda()
+    dout = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    torch.full((2 * V + 1, H), float("nan"), device="cuda", dtype=torch.bfloat16)  # leaves NaN in the memory that comes next
+    pf.embedding(ids, wte, wpe, positions=pos, sorted_grad=True).backward(dout)
+    for p, keys in ((wte, ids), (wpe, pos)):
+        value, magnitude, count = _sums(keys, dout, p.shape[0])
+        assert not p.grad[count.view(-1) == 0].any()
+        assert ((p.grad.double() - value).abs() <= (1 + U) * (count + 3) * F32 * magnitude + U * value.abs()).all()
