@@ -1,4 +1,5 @@
-// Attention over packed documents, backward, for sm_100a: two passes without atomics, the same bits on every run.
+// Attention over packed documents, backward, for sm_100a: two passes, no result is added to by
+// atomics: the same bits on every run.
 //
 //   p_ij = exp(s q_i k_j - lse_i), dp_ij = do_i v_j, ds_ij = p_ij (dp_ij - delta_i), delta_i = do_i o_i
 //   dq_i = s sum_j ds_ij k_j;  dv_j = sum_i p_ij do_i;  dk_j = s sum_i ds_ij q_i

@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(kPlanThreads) layout_kernel(LayoutArgs a) {
 // Rotates the first `heads` heads of every row ("rotate-half" pairing: element i with i + D / 2) by the row's position;
 // rows at position -1 (padding) are copied.  src and dst may be the same memory: a thread reads the 32 bytes that it
 // writes.  A block takes one row at a time, its threads the 16-byte vectors of half heads; rows are stepped by the grid, so
-// that no index is divided.  The turned values are rounded to bf16, the type that the products take them in.  Bound by bandwidth, one read and one write: 41 us for 8192 tokens of 64 heads of 128
-// elements, 6.5 TB/s.
+// that no index is divided.  The turned values are rounded to bf16, the type that the products take them in.  Bound by
+// bandwidth, one read and one write: 41 us for 8192 tokens of 64 heads of 128 elements, 6.5 TB/s.
 __global__ void __launch_bounds__(256) packed_rope_kernel(const __nv_bfloat16* src, long long src_stride,
                                                           __nv_bfloat16* dst, long long dst_stride,
                                                           const float* __restrict__ cs, const float* __restrict__ sn,
