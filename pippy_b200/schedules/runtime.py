@@ -247,8 +247,6 @@ class PipelineSchedule:
             raise TypeError(f"losses must be a list but got a {type(losses)}")
         return arg_mbs, kwarg_mbs
 
-    _shared_kwarg_mbs: Optional[List[Dict[str, Any]]] = None  # keyword arguments of every stage, per microbatch, during a step
-
     def _split_inputs(self, args: Tuple[Any, ...], kwargs: Optional[Dict[str, Any]]):
         if args or kwargs:
             args_split, kwargs_split = split_args_kwargs_into_chunks(
@@ -302,9 +300,11 @@ class PipelineSchedule:
                         f"({type(e).__name__}: {e})"
                     ) from e
 
-    def _step_microbatches(self, arg_mbs=None, kwarg_mbs=None, target_mbs=None, losses=None) -> None:
+    def _step_microbatches(self, arg_mbs=None, kwarg_mbs=None, target_mbs=None, losses=None,
+                           shared_kwarg_mbs: Optional[List[Dict[str, Any]]] = None) -> None:
+        """``shared_kwarg_mbs``: keyword arguments of every stage, one dict per microbatch."""
         arg_mbs, kwarg_mbs = self._check_inputs(arg_mbs, kwarg_mbs, target_mbs, losses)
-        shared = self._shared_kwarg_mbs or [{}] * self._n_microbatches
+        shared = shared_kwarg_mbs or [{}] * self._n_microbatches
         if self._actions is None:
             self._build()
         stages = self._stage_by_index
@@ -411,14 +411,12 @@ class PipelineSchedule:
             targets_split = list(torch.tensor_split(target, self._n_microbatches))
         else:
             targets_split = None
+        shared_split = None
         if stage_kwargs:
-            _, self._shared_kwarg_mbs = split_args_kwargs_into_chunks((), stage_kwargs, self._n_microbatches)
-            if len(self._shared_kwarg_mbs) != self._n_microbatches:
+            _, shared_split = split_args_kwargs_into_chunks((), stage_kwargs, self._n_microbatches)
+            if len(shared_split) != self._n_microbatches:
                 raise ValueError(f"stage_kwargs: {self._n_microbatches} microbatches do not come out of their first dimension")
-        try:
-            self._step_microbatches(args_split, kwargs_split, targets_split, losses)
-        finally:
-            self._shared_kwarg_mbs = None
+        self._step_microbatches(args_split, kwargs_split, targets_split, losses, shared_split)
         if not self.return_outputs:
             return None
         for st in self._stages:

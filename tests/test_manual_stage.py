@@ -117,3 +117,20 @@ def _two_steps(rank, world, schedule_name):
 @pytest.mark.parametrize("schedule_name", ["ScheduleGPipe", "Schedule1F1B"])
 def test_multi_input_output_stages_two_sgd_steps(schedule_name):
     run_ranks(_two_steps, 2, schedule_name)
+
+
+class Weighted(nn.Module):
+    def forward(self, x, w=None):
+        return x if w is None else x * w
+
+
+def test_refused_stage_kwargs_are_gone_in_the_next_step():
+    """Keyword arguments of every stage belong to the step that they were given to, also where that step was refused."""
+    stage = pp.ManualPipelineStage(Weighted(), 0, 1, torch.device("cpu"), 4, input_args=torch.empty(1, D))
+    sched = pp.ScheduleGPipe(stage, 4)
+    x, w = torch.randn(4, D), torch.randn(4, 1)
+    with pytest.raises(ValueError, match="microbatches"):
+        sched.step(x, stage_kwargs={"w": w[:2]})
+    assert torch.equal(sched.step(x), x)
+    assert torch.equal(sched.step(x, stage_kwargs={"w": w}), x * w)
+    assert torch.equal(sched.step(x), x)
