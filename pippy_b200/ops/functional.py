@@ -582,15 +582,49 @@ class _EmbeddingFn(torch.autograd.Function):
         return None, None, None, None
 
 
-# What ties the op below to autograd.  Its gradients are written by the kernels, and a table as an input would bring the
-# table's accumulation node along, which belongs to the stream of whichever graph made it: with an eager one alive, a
-# captured backward would wait for that stream.  A leaf on the CPU has no stream.
-_TIE = torch.empty(0, requires_grad=True)
+# In the place of a table that a captured graph leaves out, see below.  A leaf on the CPU has no stream.
+_NO_STREAM = torch.empty(0, device="cpu", requires_grad=True)
+_MADE_ON = "pippy_b200 stream"  # in the metadata of accumulation nodes that captured embeddings made
+
+
+def _held_elsewhere(table: torch.Tensor, stream: int) -> bool:
+    """Whether a graph that was not made on ``stream`` holds the leaf's accumulation node."""
+    node = torch.autograd.graph.get_gradient_edge(table).node  # made here where there is none
+    if _MADE_ON in node.metadata:
+        return node.metadata[_MADE_ON] != stream
+    node.metadata[_MADE_ON] = stream
+    del node  # a node that nobody else holds ends here, and what was noted on it
+    node = torch.autograd.graph.get_gradient_edge(table).node
+    return node.metadata.pop(_MADE_ON, None) is not None
+
+
+def _graph_inputs(tables):
+    """The leaves that the op below is a function of in autograd: the tables that it writes gradients for.  Their
+    accumulation nodes are what ``backward(inputs=...)``, hooks and wrappers that count ready parameters go by.
+
+    Such a node belongs to the stream on which the first of the graphs that hold it was made, and a backward waits for
+    the streams of the nodes that it reaches.  Captured, it cannot wait for a stream outside its capture: that ends the
+    process.  So a captured graph leaves a table out whose node a graph of another stream holds."""
+    if not torch.cuda.is_current_stream_capturing():
+        return tables
+    stream = torch.cuda.current_stream().cuda_stream
+    kept = [t for t in tables if not _held_elsewhere(t, stream)]
+    return kept if len(kept) == len(tables) else kept + [_NO_STREAM]
+
+
+def _note_stream(leaves) -> None:
+    """After the graph of ``leaves`` is made: a node of this capture serves the capture's later embeddings too."""
+    if torch.cuda.is_current_stream_capturing():
+        for t in leaves:
+            if t is not _NO_STREAM:
+                torch.autograd.graph.get_gradient_edge(t).node.metadata[_MADE_ON] = torch.cuda.current_stream().cuda_stream
 
 
 class _SortedEmbeddingFn(torch.autograd.Function):
+    """``leaves``: see :func:`_graph_inputs`.  The gradients of the tables are written by the kernels."""
+
     @staticmethod
-    def forward(ctx, tie, ids, tables, positions, S: int, scale: float):
+    def forward(ctx, ids, tables, positions, S: int, scale: float, *leaves):
         wte, wpe = tables
         T, H = ids.numel(), wte.shape[1]
         table, ptable = wte, wpe
@@ -624,7 +658,7 @@ class _SortedEmbeddingFn(torch.autograd.Function):
         else:
             cfg = ctx.cfg
             _run_or_defer(lambda: _embed_sorted_wgrad(ids, positions, dout, *cfg))
-        return None, None, None, None, None, None
+        return (None,) * len(ctx.needs_input_grad)
 
 
 def _embed_sorted_wgrad(ids, positions, dout, wte, wpe, S, scale):
@@ -665,7 +699,9 @@ def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 
     The tables' gradients are fp32 scatter-adds, whose order changes from run to run, unless ``sorted_grad`` is set:
     then, and always with a ``scale`` or ``positions``, tokens are sorted first and the rows of a token added in their
     order, the same bits on every run.  On that path ids outside ``wte`` and positions beyond ``wpe`` give zeros and
-    set the device error word (:func:`pippy_b200.ops._lib.check_device_errors`)."""
+    set the device error word (:func:`pippy_b200.ops._lib.check_device_errors`).  Captured while a graph made on another
+    stream (an eager one) holds a table's accumulation node, the graph leaves that table out: its gradient is written, but
+    ``backward(inputs=...)`` does not count it and hooks on it do not run."""
     S = ids.shape[-1] if seq_len is None else seq_len
     plain = scale == 1.0 and positions is None
     if positions is not None:
@@ -694,8 +730,14 @@ def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 
                 positions = positions.long().clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()
         if ids.dtype != torch.int64 or not ids.is_contiguous():
             ids = ids.long().contiguous()
-        return _SortedEmbeddingFn.apply(_TIE if trained else None, ids, (wte, wpe), positions,
-                                        S if ids.numel() else 1, float(scale))
+        S = S if ids.numel() else 1
+        if not (trained and torch.is_grad_enabled()):
+            return _SortedEmbeddingFn.apply(ids, (wte, wpe), positions, S, float(scale))
+        with _on_device_of(wte):
+            leaves = _graph_inputs(trained)
+            out = _SortedEmbeddingFn.apply(ids, (wte, wpe), positions, S, float(scale), *leaves)
+            _note_stream(leaves)
+        return out
     if plain:
         out = F.embedding(ids.reshape(-1), wte)
         if wpe is not None:

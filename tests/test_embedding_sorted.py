@@ -271,3 +271,109 @@ def test_kernel_writes_the_rows_that_do_not_occur(V, H, T, errors):
         value, magnitude, count = _sums(keys, dout, p.shape[0])
         assert not p.grad[count.view(-1) == 0].any()
         assert ((p.grad.double() - value).abs() <= (1 + U) * (count + 3) * F32 * magnitude + U * value.abs()).all()
+
+
+# ------------------------------------------------------------------------------------------------ place in the graph
+def test_whose_accumulation_nodes_are_held_elsewhere():
+    leaf = torch.nn.Parameter(torch.ones(3))
+    assert not pf._held_elsewhere(leaf, 1) and not pf._held_elsewhere(leaf, 1)
+    graph = leaf * 2
+    assert pf._held_elsewhere(leaf, 1) and pf._held_elsewhere(leaf, 1)
+    del graph
+    assert not pf._held_elsewhere(leaf, 1)
+    graph = leaf * 2
+    torch.autograd.graph.get_gradient_edge(leaf).node.metadata[pf._MADE_ON] = 1
+    assert not pf._held_elsewhere(leaf, 1) and pf._held_elsewhere(leaf, 2)
+    del graph
+
+
+def _tables(V=50, P=100, H=64, T=300):
+    ids, gen = _ids(T, V, 0.2)
+    wte, wpe = (torch.nn.Parameter(torch.randn(n, H, generator=gen).bfloat16().cuda()) for n in (V, P))
+    return ids, wte, wpe, torch.randn(T, H, generator=gen).bfloat16().cuda()
+
+
+@gpu
+@pytest.mark.parametrize("buffers", [False, True])
+def test_kernel_gradients_of_chosen_inputs_and_hooks(buffers, errors):
+    """What goes by the tables' accumulation nodes: ``inputs=`` of a backward, and hooks."""
+    ids, wte, wpe, dout = _tables()
+    want = [_sums(ids, dout, 50), _sums(torch.arange(300, device="cuda") % 100, dout, 100)]
+    seen = []
+    for p in (wte, wpe):
+        p.register_post_accumulate_grad_hook(seen.append)
+
+    def check(chosen):
+        for p, (value, magnitude, count) in zip((wte, wpe), want):
+            got = p.main_grad if buffers else p.grad
+            if any(p is q for q in chosen):
+                assert ((got.double() - value).abs() <= (1 + U) * (count + 3) * F32 * magnitude + U * value.abs()).all()
+        assert len(seen) == len(chosen) and all(any(p is q for q in seen) for p in chosen)
+
+    for chosen in ([wte, wpe], [wte], [wpe]):
+        for p in (wte, wpe):
+            p.grad = None
+            if buffers:
+                p.main_grad = torch.zeros(p.shape, device="cuda")
+        seen.clear()
+        pf.embedding(ids, wte, wpe, 100, sorted_grad=True).backward(dout, inputs=chosen)
+        check(chosen)
+
+
+@gpu
+def test_kernel_captured_gradients_of_chosen_inputs(errors):
+    """Without another graph of the tables, a captured one has them as inputs: two at a time, and one capture after another."""
+    ids, wte, wpe, dout = _tables()
+    for p in (wte, wpe):
+        p.main_grad = torch.zeros(p.shape, device="cuda")
+    pf.embedding(ids, wte, wpe, 100, sorted_grad=True).backward(dout)
+    want = [2 * p.main_grad for p in (wte, wpe)]  # exactly: two equal sums
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            for p in (wte, wpe):
+                p.main_grad.zero_()
+            outs = [pf.embedding(ids, wte, wpe, 100, sorted_grad=True) for _ in range(2)]
+            for out in outs:
+                out.backward(dout, inputs=[wte, wpe])
+        graphs.append((graph, outs))
+    for graph, _ in graphs:
+        for p in (wte, wpe):
+            p.main_grad.fill_(3.0)
+        graph.replay()
+        assert all(torch.equal(p.main_grad, w) for p, w in zip((wte, wpe), want))
+
+
+def _ddp(rank, world):
+    from torch.nn.parallel import DistributedDataParallel
+
+    from pippy_b200.models.gpt2 import GPT2Config, GPT2Stage
+
+    torch.cuda.set_device(0)
+    cfg = GPT2Config(vocab_size=300, n_positions=128, dim=128, n_layers=1, n_heads=2)
+    torch.manual_seed(0)
+    model = GPT2Stage(cfg, range(1), True, True, device="cuda", dtype=torch.bfloat16)
+    ids, lengths = torch.randint(0, 300, (2, 128), device="cuda"), torch.tensor([[100, 28], [40, 60]], device="cuda")
+    g = torch.randn(2, 128, cfg.padded_vocab, device="cuda").bfloat16()
+
+    def grads(m):
+        for p in model.parameters():
+            p.grad = None
+        m(ids, lengths=lengths).backward(g)
+        torch.cuda.synchronize()
+        return [p.grad.clone() for p in model.parameters()]
+
+    want = grads(model)
+    wrapped = DistributedDataParallel(model, device_ids=[0])
+    for _ in range(2):  # a parameter that was never counted as ready shows in the second step
+        for a, b in zip(grads(wrapped), want):
+            assert (a - b).norm() <= 2 * U * b.norm()  # the same sums, each rounded once, whatever their order
+
+
+@gpu
+def test_packed_stage_in_a_data_parallel_wrapper():
+    from _mp import run_ranks
+
+    run_ranks(_ddp, 1, backend="nccl")
