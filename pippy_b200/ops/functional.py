@@ -663,32 +663,34 @@ class _SortedEmbeddingFn(torch.autograd.Function):
 
 def _embed_sorted_wgrad(ids, positions, dout, wte, wpe, S, scale):
     T, H = dout.shape
-    params = [p for p in (wte, wpe) if p is not None and p.requires_grad]
-
-    def has_buffer(p):
+    # a table with an fp32 buffer has the sums added in fp32, any other gets its gradient whole, in its own type
+    added, written = {}, {}
+    for p in (wte, wpe):
+        if p is None or not p.requires_grad:
+            continue
         mg = getattr(p, "main_grad", None)
-        return mg is not None and mg.dtype == torch.float32 and mg.is_contiguous() and mg.data_ptr() % 16 == 0
-
-    # the kernel adds to the parameters' fp32 buffers, or it writes gradients whole, in the parameters' type
-    direct = all(map(has_buffer, params))
-    grads = [p.main_grad if direct else torch.empty(p.shape, dtype=p.dtype, device=p.device) for p in params]
-    gw = grads[0].data_ptr() if wte.requires_grad else None
-    gp = grads[-1].data_ptr() if wpe is not None and wpe.requires_grad else None
+        if mg is None or mg.dtype != torch.float32:
+            written[p] = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+        else:
+            fits = mg.is_contiguous() and mg.data_ptr() % 16 == 0
+            added[p] = mg if fits else torch.zeros(p.shape, dtype=torch.float32, device=p.device)
     lib = _lib.lib()
-    scratch = torch.empty(lib.pb_embed_sorted_scratch(T, H, len(params)), dtype=torch.uint8, device=dout.device)
     with _on_device_of(dout):
-        _lib.check(
-            lib.pb_embed_sorted_bwd(ids.data_ptr(), _lib.addr(positions), dout.data_ptr(), gw, gp, T, H, S, wte.shape[0],
-                                    0 if wpe is None else wpe.shape[0], scale, int(not direct), scratch.data_ptr(),
-                                    _lib.stream_addr()),
-            "pb_embed_sorted_bwd",
-        )
-        if not direct:
-            for p, g in zip(params, grads):
-                if getattr(p, "main_grad", None) is None and p.grad is None:
-                    p.grad = g
-                else:
-                    _accumulate_param_grad(p, g)
+        for grads in (added, written):
+            if not grads:
+                continue
+            scratch = torch.empty(lib.pb_embed_sorted_scratch(T, H, len(grads)), dtype=torch.uint8, device=dout.device)
+            _lib.check(
+                lib.pb_embed_sorted_bwd(ids.data_ptr(), _lib.addr(positions), dout.data_ptr(), _lib.addr(grads.get(wte)),
+                                        _lib.addr(grads.get(wpe)), T, H, S, wte.shape[0], 0 if wpe is None else wpe.shape[0],
+                                        scale, int(grads is written), scratch.data_ptr(), _lib.stream_addr()),
+                "pb_embed_sorted_bwd",
+            )
+        for p, g in (*added.items(), *written.items()):
+            if getattr(p, "main_grad", None) is None and p.grad is None:
+                p.grad = g
+            elif g is not getattr(p, "main_grad", None):
+                _accumulate_param_grad(p, g)
 
 
 def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 1.0,

@@ -377,3 +377,25 @@ def test_packed_stage_in_a_data_parallel_wrapper():
     from _mp import run_ranks
 
     run_ranks(_ddp, 1, backend="nccl")
+
+
+@gpu
+@pytest.mark.parametrize("which", ["wte", "wpe", "unaligned", "strided"])
+def test_kernel_keeps_fp32_for_the_table_that_has_a_buffer(which, errors):
+    """One table with an fp32 buffer and one without; buffers that the kernel cannot add to: no rounding to bf16 on the way."""
+    ids, wte, wpe, dout = _tables()
+    want = [_sums(ids, dout, 50), _sums(torch.arange(300, device="cuda") % 100, dout, 100)]
+    for p, name in ((wte, "wte"), (wpe, "wpe")):
+        if which == "unaligned":
+            p.main_grad = torch.zeros(p.numel() + 1, device="cuda")[1:].view(p.shape)
+        elif which == "strided":
+            p.main_grad = torch.zeros(p.shape[0], 2 * p.shape[1], device="cuda")[:, : p.shape[1]]
+        elif which == name:
+            p.main_grad = torch.zeros(p.shape, device="cuda")
+    pf.embedding(ids, wte, wpe, 100, sorted_grad=True).backward(dout)
+    for p, (value, magnitude, count) in zip((wte, wpe), want):
+        bound = (count + 3) * F32 * magnitude
+        if hasattr(p, "main_grad"):
+            assert p.grad is None and ((p.main_grad.double() - value).abs() <= bound).all()
+        else:
+            assert ((p.grad.double() - value).abs() <= (1 + U) * bound + U * value.abs()).all()
