@@ -68,8 +68,9 @@ class GPT2Block(nn.Module):
         self.mlp_c_fc = Linear(d, 4 * d, bias=True, init_std=cfg.init_std, device=device, dtype=dtype)
         self.mlp_c_proj = Linear(4 * d, d, bias=True, init_std=cfg.init_std, device=device, dtype=dtype)
 
-    def forward(self, x, B: int, S: int, layout=None, seed=None):
-        """``layout``: documents in the rows.  ``seed``: of the stage's dropout masks; the block's index tells them apart."""
+    def forward(self, x, B: int, S: int, layout=None, seed=None, stream: int = 0):
+        """``layout``: documents in the rows.  ``seed``: of the stage's dropout masks; ``stream`` and the block's index tell
+        them apart."""
         cfg = self.cfg
         qkv = self.attn_c_attn(self.ln_1(x))
         if layout is None:
@@ -79,11 +80,11 @@ class GPT2Block(nn.Module):
         if seed is None:
             x = self.attn_c_proj(att, residual=x)
         else:
-            x = self.drop(self.attn_c_proj(att), residual=x, seed=seed, stream=2 * self.index + 1)
+            x = self.drop(self.attn_c_proj(att), residual=x, seed=seed, stream=stream + 2 * self.index + 1)
         h = self.mlp_c_fc(self.ln_2(x), activation="gelu_tanh")
         if seed is None:
             return self.mlp_c_proj(h, residual=x)
-        return self.drop(self.mlp_c_proj(h), residual=x, seed=seed, stream=2 * self.index + 2)
+        return self.drop(self.mlp_c_proj(h), residual=x, seed=seed, stream=stream + 2 * self.index + 2)
 
 
 class GPT2Stage(nn.Module):
@@ -92,7 +93,10 @@ class GPT2Stage(nn.Module):
 
     ``lengths`` ([B, documents], see ``pf.packed_layout``): the rows hold documents, which do not see one another and
     whose positions begin at 0; every stage gets it.  With ``cfg.dropout`` a training forward draws one seed from the
-    device's default generator (data-parallel ranks seed theirs differently)."""
+    device's default generator; ``replica`` (the data-parallel rank; ``train.build_gpt2_pipeline`` sets it) keeps the masks of
+    replicas apart whose generators are in the same state, as they are after equal initialisation."""
+
+    replica: int = 0
 
     def __init__(self, cfg: GPT2Config, layer_ids, first: bool, last: bool, device=None, dtype=None):
         super().__init__()
@@ -116,14 +120,15 @@ class GPT2Stage(nn.Module):
         B, S = x.shape[:2]
         layout = None if lengths is None else batch_layout(lengths, B, S)
         seed = Dropout.draw(x.device) if self.training and self.cfg.dropout > 0.0 else None
+        stream = self.replica << 32  # of the replica's first mask; a replica has fewer than 2^32 of them
         if self.first:
             h = self.wte(x, None if layout is None else layout.positions)
             if seed is not None:
-                h = self.drop(h, seed=seed)
+                h = self.drop(h, seed=seed, stream=stream)
         else:
             h = x.reshape(B * S, -1)
         for blk in self.h.values():
-            h = blk(h, B, S, layout, seed)
+            h = blk(h, B, S, layout, seed, stream)
         if self.last:
             h = pf.linear(self.ln_f(h), self.head_weight())
         return h.view(B, S, -1)

@@ -200,6 +200,7 @@ def build_gpt2_pipeline(
     for s in held:
         torch.manual_seed(seed + s)
         module = build_gpt2_stage(cfg, s, num_stages, device=device, dtype=dtype, balance=balance)
+        module.replica = 0 if dp_group is None else dist.get_rank(dp_group)
         inp = (torch.empty(mb, seq_len, dtype=torch.int64, device="meta") if s == 0
                else torch.empty(mb, seq_len, cfg.dim, dtype=dtype, device="meta"))
         out = (torch.empty(mb, seq_len, cfg.padded_vocab, dtype=dtype, device="meta") if s == num_stages - 1

@@ -161,3 +161,40 @@ def test_kernel_beyond_32_bits():
     del x, y
     torch.cuda.empty_cache()
     assert _lib.lib().pb_dropout(None, None, None, -1, None, 0, 0, 0, None) == -1
+
+
+def _replica_masks(rank, world):
+    import torch.distributed as dist
+
+    from pippy_b200.models.gpt2 import GPT2Config
+    from pippy_b200.parallel.mesh import init_mesh
+    from pippy_b200.train import build_gpt2_pipeline
+
+    mesh = init_mesh(dp_size=world)
+    cfg = GPT2Config(vocab_size=60, n_positions=16, dim=32, n_layers=2, n_heads=2, vocab_multiple=8, dropout=0.5)
+    pipe = build_gpt2_pipeline(cfg, 4, 16, 2, torch.device("cpu"), group=mesh.pp_group, dp_group=mesh.dp_group,
+                               dtype=torch.float32, lr=0.0, weight_decay=0.0)
+    drawn, original = [], pf.dropout
+
+    def record(x, p, seed, residual=None, stream=0):
+        drawn.append(original(torch.ones(64), p, seed, stream=stream).tolist())
+        return original(x, p, seed, residual=residual, stream=stream)
+
+    weights = torch.cat([p.detach().reshape(-1) for p in pipe.stages[0].submod.parameters()]).tolist()
+    ids = torch.randint(0, 60, (4, 16), generator=torch.Generator().manual_seed(1))
+    pf.dropout = record
+    try:
+        pipe.train_step(ids, ids)
+    finally:
+        pf.dropout = original
+    replicas = [None] * world
+    dist.all_gather_object(replicas, (weights, drawn))
+    assert replicas[0][0] == replicas[1][0]  # the same model
+    masks = [tuple(m) for _, ms in replicas for m in ms]
+    assert len(masks) == 2 * 2 * 5 and len(set(masks)) == len(masks)  # 2 microbatches of embedding and 2 masks a block
+
+
+def test_data_parallel_replicas_draw_masks_of_their_own():
+    from _mp import run_ranks
+
+    run_ranks(_replica_masks, 2)
