@@ -69,9 +69,10 @@ def sm_count() -> int:
 def _accumulate_param_grad(param: torch.Tensor, grad: torch.Tensor) -> None:
     mg = getattr(param, "main_grad", None)
     if mg is not None:
-        if grad.dtype == torch.bfloat16 and mg.dtype == torch.float32 and grad.is_cuda and grad.numel() % 8 == 0:
+        if grad.dtype == torch.bfloat16 and mg.dtype == torch.float32 and grad.is_cuda and grad.numel() % 8 == 0 and \
+                mg.is_contiguous() and mg.data_ptr() % 16 == 0:  # the kernel adds 16 bytes at a time, row by row
             _lib.check(
-                _lib.lib().pb_accum_bf16_into_f32(_lib.addr(mg), _lib.addr(grad.contiguous()), grad.numel(),
+                _lib.lib().pb_accum_bf16_into_f32(_lib.addr(mg), _lib.addr(_aligned(grad)), grad.numel(),
                                                   _lib.stream_addr()),
                 "pb_accum_bf16_into_f32",
             )

@@ -399,3 +399,20 @@ def test_kernel_keeps_fp32_for_the_table_that_has_a_buffer(which, errors):
             assert p.grad is None and ((p.main_grad.double() - value).abs() <= bound).all()
         else:
             assert ((p.grad.double() - value).abs() <= (1 + U) * bound + U * value.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("which", ["aligned", "unaligned", "strided", "unaligned_gradient"])
+def test_adding_bf16_gradients_to_fp32_buffers_of_any_layout(which, errors):
+    p = torch.nn.Parameter(torch.zeros(24, 16, device="cuda").bfloat16())
+    room = torch.zeros(2 * p.numel() + 1, device="cuda")
+    p.main_grad = {"aligned": room[: p.numel()].view(p.shape), "unaligned": room[1 : p.numel() + 1].view(p.shape),
+                   "strided": room[: 2 * p.numel()].view(24, 32)[:, :16],
+                   "unaligned_gradient": room[: p.numel()].view(p.shape)}[which]
+    p.main_grad.fill_(1.0)
+    g = torch.randn(p.numel() + 1, device="cuda").bfloat16()
+    g = (g[1:] if which == "unaligned_gradient" else g[:-1]).view(p.shape)
+    outside = room.sum() - p.main_grad.sum()
+    pf._accumulate_param_grad(p, g)
+    assert torch.equal(p.main_grad, 1.0 + g.float()) and p.grad is None
+    assert outside == 0 and (room != 0).sum() <= p.numel()
