@@ -41,11 +41,13 @@ struct Comm {
 constexpr int MAX_EXPERTS = 16;
 constexpr int ROUTE_THREADS = 256;
 
-// One thread per token.  logits: [T, ld] bf16.  Outputs: probs [T, E] fp32, topi / topw [T, k] (weights normalised
+// One thread per token.  logits: [T, ld] bf16; positions [T] (may be null): rows at -1 are padding, which is not routed
+// (topi -1, topw and probs 0) and not counted.  Outputs: probs [T, E] fp32, topi / topw [T, k] (weights normalised
 // over the selected k), pos [T*k] = rank of the assignment among this CTA's assignments to the same expert (token
 // order), cta_counts / cta_psum [gridDim.x, E] = this CTA's assignments per expert and sums of probabilities.
 __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const __nv_bfloat16* __restrict__ logits, int ld,
-                                                                  int T, int E, int k, float* __restrict__ probs,
+                                                                  const int* __restrict__ positions, int T, int E,
+                                                                  int k, float* __restrict__ probs,
                                                                   int* __restrict__ topi, float* __restrict__ topw,
                                                                   int* __restrict__ pos, int* __restrict__ cta_counts,
                                                                   float* __restrict__ cta_psum) {
@@ -53,7 +55,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const __nv_bfl
   __shared__ float s_wsum[ROUTE_THREADS / 32][MAX_EXPERTS];
   const int t = blockIdx.x * ROUTE_THREADS + threadIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool live = t < T;
+  const bool live = t < T && (positions == nullptr || positions[t] >= 0);
   float p[MAX_EXPERTS];
   int sel[MAX_TOPK];
   unsigned chosen = 0;
@@ -102,7 +104,16 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const __nv_bfl
       }
   } else {
 #pragma unroll
-    for (int e = 0; e < MAX_EXPERTS; ++e) p[e] = 0.f;
+    for (int e = 0; e < MAX_EXPERTS; ++e) {
+      p[e] = 0.f;
+      if (t < T && e < E) probs[(long long)t * E + e] = 0.f;
+    }
+    if (t < T)
+      for (int j = 0; j < k; ++j) {
+        topi[(long long)t * k + j] = -1;
+        topw[(long long)t * k + j] = 0.f;
+        pos[(long long)t * k + j] = 0;
+      }
   }
   // per expert: how many tokens of this warp chose it, and which of them come before this token
   int rank_in_warp[MAX_EXPERTS];
@@ -146,17 +157,19 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const __nv_bfl
 }
 
 // One CTA: prefix over the route kernel's CTAs (in order), totals, the load-balance loss, final positions.
-//   counts[e] = assignments to e; share[e] = counts[e] / (T k); aux = E * sum_e share[e] * mean_t probs[t, e]
+//   counts[e] = assignments to e; share[e] = counts[e] / (n k); aux = E * sum_e share[e] * sum_t probs[t, e] / n, n the
+//   tokens that are routed, which share[E] keeps for the backward.
 __global__ void __launch_bounds__(1024) moe_route_finish_kernel(int* __restrict__ cta_counts,
                                                                 const float* __restrict__ cta_psum, int n_cta, int T,
                                                                 int E, int k, const int* __restrict__ topi,
                                                                 int* __restrict__ pos, int* __restrict__ counts,
                                                                 float* __restrict__ share, float* __restrict__ aux) {
   __shared__ float s_term[MAX_EXPERTS];
+  __shared__ int s_run[MAX_EXPERTS];
+  int run = 0;
+  float ps = 0.f;
   if (threadIdx.x < E) {
     const int e = threadIdx.x;
-    int run = 0;
-    float ps = 0.f;
     for (int c = 0; c < n_cta; ++c) {
       const int v = cta_counts[c * E + e];
       cta_counts[c * E + e] = run;  // becomes the CTA's base
@@ -164,9 +177,16 @@ __global__ void __launch_bounds__(1024) moe_route_finish_kernel(int* __restrict_
       ps += cta_psum[c * E + e];
     }
     counts[e] = run;
-    const float sh = (float)run / (float)((long long)T * k);
-    share[e] = sh;
-    s_term[e] = sh * (ps / (float)T);
+    s_run[e] = run;
+  }
+  __syncthreads();
+  if (threadIdx.x < E) {
+    long long all = 0;  // assignments: k for each token that is routed
+    for (int e = 0; e < E; ++e) all += s_run[e];
+    const float sh = all ? (float)run / (float)all : 0.f;
+    share[threadIdx.x] = sh;
+    s_term[threadIdx.x] = all ? sh * (ps / (float)(all / k)) : 0.f;
+    if (threadIdx.x == 0) share[E] = (float)(all / k);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -176,10 +196,11 @@ __global__ void __launch_bounds__(1024) moe_route_finish_kernel(int* __restrict_
   }
   const long long n = (long long)T * k;
   for (long long a = threadIdx.x; a < n; a += blockDim.x)
-    pos[a] += cta_counts[(int)((a / k) / ROUTE_THREADS) * E + topi[a]];
+    if (topi[a] >= 0) pos[a] += cta_counts[(int)((a / k) / ROUTE_THREADS) * E + topi[a]];
 }
 
-// dlogits[t, :] from g_w [T, k] (gradient of the normalised top-k weights) and *g_aux (gradient of the aux loss).
+// dlogits[t, :] from g_w [T, k] (gradient of the normalised top-k weights) and *g_aux (gradient of the aux loss); zeros where t is
+// not routed.
 __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_bwd_kernel(const float* __restrict__ probs,
                                                                       const int* __restrict__ topi,
                                                                       const float* __restrict__ topw,
@@ -190,12 +211,16 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_bwd_kernel(const floa
                                                                       int ld) {
   const int t = blockIdx.x * ROUTE_THREADS + threadIdx.x;
   if (t >= T) return;
+  if (topi[(long long)t * k] < 0) {
+    for (int e = 0; e < ld; ++e) dlogits[(long long)t * ld + e] = __float2bfloat16(0.f);
+    return;
+  }
   float p[MAX_EXPERTS], dp[MAX_EXPERTS];
   const float ga = g_aux ? *g_aux : 0.f;
 #pragma unroll
   for (int e = 0; e < MAX_EXPERTS; ++e) {
     p[e] = e < E ? probs[(long long)t * E + e] : 0.f;
-    dp[e] = e < E ? ga * (float)E * share[e] / (float)T : 0.f;
+    dp[e] = e < E ? ga * (float)E * share[e] / share[E] : 0.f;
   }
   if (g_w) {
     float s = 0.f, gdotw = 0.f;
@@ -244,7 +269,7 @@ constexpr int ERR_CAPACITY = 4;
 // count table (row s = what rank s holds); recv[r]: every rank's receive buffer [cap_rows, H]; scale: optional [T*k]
 // fp32.  Outputs on this rank: dst_base[e] = first row of this rank's block inside expert e's group on its owner
 // (what the combine needs), group_rows / group_start [experts_per_rank] = the layout of this rank's own receive
-// buffer (what the grouped GEMM needs), rows_used = where the last group's padding ends.
+// buffer (what the grouped GEMM needs), rows_used = where the last group's padding ends.  Expert -1: no assignment.
 __global__ void __launch_bounds__(THREADS) moe_dispatch_kernel(const __nv_bfloat16* __restrict__ x,
                                                                const int* __restrict__ expert,
                                                                const int* __restrict__ slot,
@@ -311,6 +336,7 @@ __global__ void __launch_bounds__(THREADS) moe_dispatch_kernel(const __nv_bfloat
   const long long n = (long long)T * k;
   for (long long a = blockIdx.x * warps_per_block + warp; a < n; a += (long long)gridDim.x * warps_per_block) {
     const int e = expert[a];
+    if (e < 0) continue;
     const int d = e / experts_per_rank;
     const long long row = (long long)s_base[e] + slot[a];
     if (row >= cap_rows) continue;
@@ -343,7 +369,7 @@ __global__ void __launch_bounds__(THREADS) moe_dispatch_kernel(const __nv_bfloat
   handshake(c, 1);  // everything destined to me has landed when every peer reports "pushed"
 }
 
-// out[t] = sum_k w[t,k] * y[d(t,k)][row(t,k)]; rowmap: [T*k] row inside the owner's buffer; optional save [T*k, H].
+// out[t] = sum_k w[t,k] * y[d(t,k)][row(t,k)], expert -1 contributes zeros; optional save [T*k, H].
 __global__ void __launch_bounds__(THREADS) moe_combine_kernel(__nv_bfloat16* __restrict__ out,
                                                               const int* __restrict__ expert,
                                                               const int* __restrict__ slot,
@@ -368,13 +394,13 @@ __global__ void __launch_bounds__(THREADS) moe_combine_kernel(__nv_bfloat16* __r
       if (j < k) {
         const long long a = t * k + j;
         const int e = expert[a];
-        long long row = (long long)dst_base[e] + slot[a];
+        rows[j] = nullptr;
         w[j] = weight ? weight[a] : 1.f;
-        if (row >= cap_rows) {  // the dispatch dropped this row (receive buffer full, error word set): contributes 0
-          row = 0;
-          w[j] = 0.f;
+        if (e >= 0) {
+          const long long row = (long long)dst_base[e] + slot[a];
+          // beyond the capacity: the dispatch dropped this row (receive buffer full, error word set)
+          if (row < cap_rows) rows[j] = reinterpret_cast<const uint4*>(s_y[e / experts_per_rank] + row * H);
         }
-        rows[j] = reinterpret_cast<const uint4*>(s_y[e / experts_per_rank] + row * H);
       }
     }
     // peer loads take microseconds: every lane issues k * UNROLL of them before it touches the first result
@@ -384,7 +410,7 @@ __global__ void __launch_bounds__(THREADS) moe_combine_kernel(__nv_bfloat16* __r
       for (int j = 0; j < MAX_TOPK; ++j)
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i)
-          if (j < k && v0 + i * 32 < vec) u[j][i] = rows[j][v0 + i * 32];
+          if (j < k && v0 + i * 32 < vec) u[j][i] = rows[j] ? rows[j][v0 + i * 32] : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < UNROLL; ++i) {
         if (v0 + i * 32 >= vec) continue;
@@ -453,16 +479,18 @@ static Comm make_comm(int** flags, int* counter, int* err, int rank, int world, 
 extern "C" {
 
 // Router: logits [T, ld] bf16 -> probs [T, E], topi / topw [T, k], slot [T*k] (position inside the expert's group of
-// this rank's assignments, token order), counts [E], share [E], aux (scalar).  scratch_i: int[n_cta * E],
-// scratch_f: float[n_cta * E] with n_cta = ceil(T / 256).  E <= 16, k <= 4.
-int pb_moe_route(const void* logits, int ld, int T, int E, int k, float* probs, int* topi, float* topw, int* slot,
-                 int* counts, float* share, float* aux, int* scratch_i, float* scratch_f, void* stream_) {
+// this rank's assignments, token order), counts [E], share [E + 1] (the last: how many tokens are routed), aux (scalar).
+// positions [T] int32, may be null: rows at -1 are not routed.  scratch_i: int[n_cta * E], scratch_f: float[n_cta * E]
+// with n_cta = ceil(T / 256).  E <= 16, k <= 4.
+int pb_moe_route(const void* logits, int ld, const int* positions, int T, int E, int k, float* probs, int* topi,
+                 float* topw, int* slot, int* counts, float* share, float* aux, int* scratch_i, float* scratch_f,
+                 void* stream_) {
   using namespace pbmoe;
   if (E < 1 || E > MAX_EXPERTS || k < 1 || k > MAX_TOPK || k > E || ld < E || T < 1) return -1;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const int n_cta = (T + ROUTE_THREADS - 1) / ROUTE_THREADS;
-  moe_route_kernel<<<n_cta, ROUTE_THREADS, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(logits), ld, T, E, k,
-                                                        probs, topi, topw, slot, scratch_i, scratch_f);
+  moe_route_kernel<<<n_cta, ROUTE_THREADS, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(logits), ld, positions,
+                                                        T, E, k, probs, topi, topw, slot, scratch_i, scratch_f);
   moe_route_finish_kernel<<<1, 1024, 0, stream>>>(scratch_i, scratch_f, n_cta, T, E, k, topi, slot, counts, share,
                                                   aux);
   pb_count_launch(2);

@@ -45,7 +45,8 @@ class MixtralBlock(nn.Module):
 
     def forward(self, x, B: int, S: int, layout=None):
         x = self.attention(self.attention_norm(x), x, B, S, layout)
-        return x + self.block_sparse_moe(self.ffn_norm(x))
+        # padding is not routed
+        return x + self.block_sparse_moe(self.ffn_norm(x), None if layout is None else layout.positions)
 
 
 class MixtralStage(nn.Module):

@@ -123,7 +123,7 @@ class _Plan:
         self.expert = torch.empty(T * k, dtype=torch.int32, device=dev)   # expert of assignment (t, j)
         self.slot = torch.empty(T * k, dtype=torch.int32, device=dev)     # its position among this rank's rows for that expert
         self.counts = torch.empty(E, dtype=torch.int32, device=dev)       # this rank's rows per expert
-        self.share = torch.empty(E, dtype=torch.float32, device=dev)
+        self.share = torch.empty(E + 1, dtype=torch.float32, device=dev)  # of the assignments; last: tokens routed
         self.dst_base = torch.empty(E, dtype=torch.int32, device=dev)     # filled by the dispatch kernel
         self.group_rows = torch.zeros(ep.experts_per_rank, dtype=torch.int32, device=dev)
         self.group_start = torch.zeros(ep.experts_per_rank, dtype=torch.int32, device=dev)
@@ -132,10 +132,10 @@ class _Plan:
 
 class _RouteFn(torch.autograd.Function):
     """logits [T, E_pad] -> (normalised top-k weights [T, k] fp32, load-balance loss); indices, positions and counts
-    go into ``plan``."""
+    go into ``plan``.  ``positions``: int32 [T], rows at -1 are not routed (expert -1)."""
 
     @staticmethod
-    def forward(ctx, logits, plan: _Plan, E: int, k: int):
+    def forward(ctx, logits, plan: _Plan, E: int, k: int, positions=None):
         T, ld = logits.shape
         dev = logits.device
         probs = torch.empty(T, E, dtype=torch.float32, device=dev)
@@ -145,7 +145,7 @@ class _RouteFn(torch.autograd.Function):
         scratch_i = torch.empty(n_cta * E, dtype=torch.int32, device=dev)
         scratch_f = torch.empty(n_cta * E, dtype=torch.float32, device=dev)
         _lib.check(_lib.lib().pb_moe_route(
-            _lib.ptr(logits), _lib.c_int(ld), _lib.c_int(T), _lib.c_int(E), _lib.c_int(k), _lib.ptr(probs),
+            _lib.ptr(logits), _lib.c_int(ld), _lib.ptr(positions), _lib.c_int(T), _lib.c_int(E), _lib.c_int(k), _lib.ptr(probs),
             _lib.ptr(plan.expert), _lib.ptr(topw), _lib.ptr(plan.slot), _lib.ptr(plan.counts), _lib.ptr(plan.share),
             _lib.ptr(aux), _lib.ptr(scratch_i), _lib.ptr(scratch_f), _lib.stream_ptr()), "pb_moe_route")
         ctx.save_for_backward(probs, topw)
@@ -164,7 +164,7 @@ class _RouteFn(torch.autograd.Function):
             _lib.ptr(probs), _lib.ptr(plan.expert), _lib.ptr(topw), _lib.ptr(g_w), _lib.ptr(g_aux),
             _lib.ptr(plan.share), _lib.c_int(T), _lib.c_int(E), _lib.c_int(k), _lib.ptr(dlogits), _lib.c_int(ld),
             _lib.stream_ptr()), "pb_moe_route_bwd")
-        return dlogits, None, None, None
+        return dlogits, *(None,) * (len(ctx.needs_input_grad) - 1)
 
 
 def grouped_gemm(mode: int, a, b, out, n, k_dim, plan: _Plan, b_mn: bool = False, accumulate: bool = False):
@@ -288,7 +288,10 @@ class _AuxLossInject(torch.autograd.Function):
 class MoEFeedForward(nn.Module):
     """Top-k routed SwiGLU experts. ``n_experts`` in total, this rank holds ``n_experts / ep_size`` of them
     (expert ``e`` lives on rank ``e // experts_per_rank``) as two stacked parameters ``w_gate_up [local, 2 ffn, dim]``
-    and ``w_down [local, dim, ffn]``. Input/output: ``[T, dim]``."""
+    and ``w_down [local, dim, ffn]``. Input/output: ``[T, dim]``.
+
+    ``positions`` (int32 ``[T]``, a ``pf.PackedLayout``'s): rows at -1 are padding; they go to no expert, take no room in the
+    receive buffers, do not count in the load-balance loss and come out as zeros."""
 
     def __init__(self, dim: int, ffn_dim: int, n_experts: int, top_k: int = 2, ep: Optional[EPContext] = None,
                  ep_size: int = 1, ep_rank: int = 0, aux_coef: float = 0.01, init_std: float = 0.02, device=None,
@@ -327,12 +330,16 @@ class MoEFeedForward(nn.Module):
         aux = self.n_experts * (share * probs.mean(0)).sum()
         return topw, topi, aux
 
-    def forward(self, x):
+    def forward(self, x, positions: Optional[torch.Tensor] = None):
         T = x.shape[0]
+        if positions is not None and (positions.shape != (T,) or positions.dtype != torch.int32 or positions.device != x.device):
+            raise ValueError(f"positions: int32 [{T}] on {x.device}, got {tuple(positions.shape)} {positions.dtype} on "
+                             f"{positions.device}")
         if self.ep is not None and x.is_cuda and x.dtype == torch.bfloat16:
             plan = _Plan(self.ep, T)
             logits = pf.linear(x, self.router)
-            topw, aux = _RouteFn.apply(logits, plan, self.n_experts, self.top_k)
+            positions = positions if positions is None else positions.contiguous()
+            topw, aux = _RouteFn.apply(logits, plan, self.n_experts, self.top_k, positions)
             self.last_aux_loss = aux.detach()
             if self.aux_coef:
                 x = _AuxLossInject.apply(x, aux * self.aux_coef)
@@ -343,6 +350,15 @@ class MoEFeedForward(nn.Module):
         # dense reference path (one rank holds every expert): plain PyTorch statement of the same layer
         if self.ep_size != 1:
             raise RuntimeError("the reference MoE path needs all experts on one rank")
+        if positions is None:
+            return self._dense(x)
+        inside = (positions >= 0).nonzero(as_tuple=True)[0]
+        if inside.numel() == 0:
+            self.last_aux_loss = torch.zeros((), device=x.device)
+            return torch.zeros_like(x)
+        return torch.zeros_like(x).index_copy(0, inside, self._dense(x[inside]))
+
+    def _dense(self, x):
         topw, topi, aux = self._route_reference(x)
         self.last_aux_loss = aux.detach()
         if self.aux_coef:

@@ -161,6 +161,42 @@ def test_lengths_through_a_pipeline(schedule):
     run_ranks(_train, 2, schedule)
 
 
+def _padding_free(lengths, ids, seq):
+    """The documents of ``ids``, whose rows end in padding, in one row without any: ids, lengths, and where its tokens are."""
+    inside = torch.tensor([[t < sum(row) for t in range(seq)] for row in lengths])
+    return ids[inside].unsqueeze(0), torch.tensor([[n for row in lengths for n in row]]), inside
+
+
+def test_padding_is_not_routed_to_experts():
+    """With a balance loss, a batch whose rows end in padding trains as the same documents without any."""
+    from pippy_b200.models.mixtral import MixtralConfig, MixtralStage
+
+    torch.manual_seed(0)
+    cfg = MixtralConfig(vocab_size=64, dim=32, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=48, n_experts=4, aux_coef=0.5)
+    model = MixtralStage(cfg, range(2), True, True, dtype=torch.float64)
+    ids = torch.randint(0, 60, (3, S), generator=torch.Generator().manual_seed(1))
+    ids[~_inside(LENGTHS)] = 7
+    tight, tight_lengths, inside = _padding_free(LENGTHS, ids, S)
+    g = torch.randn(int(inside.sum()), 64, dtype=torch.float64, generator=torch.Generator().manual_seed(2))
+    results = []
+    for tokens, lengths, rows in ((ids, torch.tensor(LENGTHS), inside), (tight, tight_lengths, torch.ones_like(tight).bool())):
+        model.zero_grad()
+        out = model(tokens, lengths=lengths)[rows]
+        out.backward(g)
+        results.append([out.detach(), *model.aux_losses(), *(p.grad.clone() for p in model.parameters())])
+    # fp32 inside the plain attention, router and norms: as in the test above
+    for a, b in zip(*results):
+        assert torch.allclose(a, b, rtol=1e-3, atol=1e-5)
+    model.zero_grad()
+    out = model(ids, lengths=torch.zeros(3, 1, dtype=torch.int64))  # nothing but padding
+    out.sum().backward()
+    assert out.isfinite().all() and not torch.stack(model.aux_losses()).any()
+    assert all(p.grad is None or not p.grad.any() for p in model.expert_parameters())
+    moe = model.layers["0"].block_sparse_moe
+    with pytest.raises(ValueError, match="positions"):
+        moe(torch.zeros(4, 32, dtype=torch.float64), torch.zeros(3, dtype=torch.int32))
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 def test_operators_together_on_the_gpu():
@@ -260,4 +296,98 @@ def test_packed_llama_training_step_on_the_gpu(checkpointing):
     # both sides round the same values to bf16, in tiles of other shapes: sqrt(2) times the 0.015 of the test above, twice
     assert abs(loss.item() - total) < 0.01 * total
     assert ((got - want).norm() / want.norm()).item() < 0.04
+    _lib.check_device_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,share", [(384, 0.3), (1500, 0.9), (700, 1.0), (1, 0.0), (513, 0.0)])
+def test_experts_leave_padding_out_on_the_gpu(T, share):
+    """The kernels of the expert layer with padding among the rows, whatever it holds, against the dense layer on the others."""
+    from pippy_b200.ops import _lib
+    from pippy_b200.parallel.ep import EPContext, MoEFeedForward
+
+    H, Fd, E, k = 256, 512, 4, 2
+    gen = torch.Generator().manual_seed(T)
+    inside = (torch.rand(T, generator=gen) < share).cuda()
+    n = int(inside.sum())
+    positions = torch.where(inside, 5, -1).int()
+    # room for the tokens alone
+    ep = EPContext(None, max_tokens=max(n, 1), hidden=H, top_k=k, n_experts=E, capacity_factor=1.0)
+    torch.manual_seed(5)
+    dense = MoEFeedForward(H, Fd, E, k, None, 1, 0, aux_coef=0.5, device="cuda", dtype=torch.bfloat16)
+    fused = MoEFeedForward(H, Fd, E, k, ep, 1, 0, aux_coef=0.5, device="cuda", dtype=torch.bfloat16)
+    fused.load_state_dict(dense.state_dict())
+    for p in fused.parameters():
+        p.main_grad = torch.zeros(p.shape, device="cuda")
+    x = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    x[~inside] *= 100
+    dy = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    x.requires_grad_(True)
+    out = fused(x, positions)
+    out.backward(dy)
+    assert not out[~inside].any() and not x.grad[~inside].any()
+    if n:
+        xd = x.detach()[inside].requires_grad_(True)
+        ref = dense(xd)
+        ref.backward(dy[inside])
+
+        def off(a, b):
+            return ((a.float() - b.float()).norm() / b.float().norm()).item()
+
+        # the tolerances that the layer is held to without padding
+        assert off(out[inside], ref) < 2e-2 and off(x.grad[inside], xd.grad) < 2e-2
+        assert off(fused.router.main_grad[:E], dense.router.grad[:E]) < 3e-2
+        assert off(fused.w_down.main_grad, dense.w_down.grad) < 2e-2
+        assert off(fused.w_gate_up.main_grad, dense.w_gate_up.grad) < 2e-2
+        assert abs(float(fused.last_aux_loss) - float(dense.last_aux_loss)) < 1e-3
+    else:
+        assert float(fused.last_aux_loss) == 0.0 and not any(p.main_grad.any() for p in fused.parameters())
+    _lib.check_device_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["mixtral", "tp"])
+def test_packed_mixtral_and_tensor_parallel_on_the_gpu(form):
+    """The packed forms in bf16 on the kernels against themselves in 64 bits on the CPU: outputs and gradients."""
+    from pippy_b200.ops import _lib
+
+    lengths = torch.tensor([[100, 0, 57, 3], [128, 65, 1, 0]], dtype=torch.int32)
+    S2 = 200
+    ids = torch.randint(0, 500, (2, S2), generator=torch.Generator().manual_seed(1))
+    inside = torch.tensor([[t < int(row.sum()) for t in range(S2)] for row in lengths])
+
+    def build(device, dtype):
+        torch.manual_seed(0)
+        if form == "tp":
+            from pippy_b200.models.llama import LlamaConfig
+            from pippy_b200.models.llama_tp import TPLlamaStage
+
+            cfg = LlamaConfig.tiny(vocab_size=512, dim=256, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=512)
+            return TPLlamaStage(cfg, range(2), True, True, None, 1, 0, 2, S2, dtype=dtype).to(device)
+        from pippy_b200.models.mixtral import MixtralConfig, MixtralStage
+        from pippy_b200.parallel.ep import EPContext
+
+        cfg = MixtralConfig(vocab_size=512, dim=256, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=512, n_experts=4, top_k=4)
+        ep = EPContext(None, 2 * S2, 256, 4, 4) if device == "cuda" else None
+        # all experts for each token: a top-k that a rounding tips to another expert would be no error of the kernels
+        return MixtralStage(cfg, range(2), True, True, ep, dtype=dtype).to(device)
+
+    model, exact = build("cuda", torch.bfloat16), build("cpu", torch.float64)
+    exact.load_state_dict(model.state_dict())
+    g = torch.randn(2, S2, 512, generator=torch.Generator().manual_seed(2)).bfloat16() * inside.unsqueeze(2)
+    for m, device in ((model, "cuda"), (exact, "cpu")):
+        for p in m.parameters():
+            p.grad = None
+        out = m(ids.to(device), lengths=lengths.to(device))
+        out.backward(g.to(device).to(out.dtype))
+        m.out = out.detach()
+
+    def off(a, b):
+        return ((a.double().cpu() - b).norm() / b.norm()).item()
+
+    # as in test_operators_together_on_the_gpu; routing, gather and weighted sum of the experts add 6 roundings a block:
+    # sqrt(28 + 12) 2^-9 = 0.012 forward, sqrt(80) 2^-9 = 0.0175 for a gradient.  Twice that and a little.
+    assert off(model.out[inside.cuda()], exact.out[inside]) < 0.025
+    for (name, a), b in zip(model.named_parameters(), exact.parameters()):
+        assert off(a.grad, b.grad) < 0.04, (name, off(a.grad, b.grad))
     _lib.check_device_errors()
