@@ -210,7 +210,8 @@ class _GroupedLinearFn(torch.autograd.Function):
             if mg is not None and mg.dtype == torch.float32:
                 grouped_gemm(2, dy, a, mg, K, a.shape[0], plan, accumulate=True)
             else:
-                dw = torch.empty(G, N, K, dtype=torch.bfloat16, device=a.device)
+                # the kernel leaves the blocks of experts without rows as they are
+                dw = torch.zeros(G, N, K, dtype=torch.bfloat16, device=a.device)
                 grouped_gemm(2, dy, a, dw, K, a.shape[0], plan)
                 pf._accumulate_param_grad(weight, dw)
 

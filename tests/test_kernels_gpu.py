@@ -897,3 +897,22 @@ print("bounds-check build ok", float(loss), float(ok))
     res = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stdout[-2000:] + res.stderr[-3000:]
     assert "bounds-check build ok" in res.stdout
+
+
+def test_experts_without_tokens_get_gradients_of_zero():
+    """Weights without an fp32 buffer: the gradient is written whole, also that of an expert that no token chose."""
+    from pippy_b200.parallel.ep import EPContext, MoEFeedForward
+
+    T, H, Fd, E, k = 300, 256, 512, 4, 2
+    layer = MoEFeedForward(H, Fd, E, k, EPContext(None, T, H, k, E), device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        layer.router.zero_()  # equal probabilities: every token takes the experts 0 and 1
+    x = _bf16(T, H).requires_grad_()
+    out = layer(x)
+    # NaN in the memory that comes next
+    held = [torch.full((E, 2 * Fd, H), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    held += [torch.full((E, H, Fd), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    del held
+    out.backward(_bf16(T, H))
+    for p in (layer.w_gate_up, layer.w_down):
+        assert p.grad[:2].isfinite().all() and p.grad[:2].any() and not p.grad[2:].any()
