@@ -963,10 +963,9 @@ def packed_attention(qkv, cos, sin, layout: PackedLayout, Hq: int, Hkv: int, D: 
 # ------------------------------------------------------------------------------------------------
 # dropout
 # ------------------------------------------------------------------------------------------------
-def _philox_numbers(seed: int, stream: int, count: int, device) -> torch.Tensor:
-    """``count`` 16-bit numbers as ``csrc/dropout.cu`` draws them, in 64-bit integer arithmetic."""
+def _philox_blocks(seed: int, stream: int, block: torch.Tensor) -> torch.Tensor:
+    """The eight 16-bit numbers of each numbered block of elements, in 64-bit integer arithmetic."""
     low = 0xFFFFFFFF
-    block = torch.arange((count + 7) // 8, device=device)
     x = [block & low, block >> 32, torch.full_like(block, stream & low), torch.full_like(block, (stream >> 32) & low)]
     k0, k1 = seed & low, (seed >> 32) & low
     for _ in range(10):
@@ -974,7 +973,12 @@ def _philox_numbers(seed: int, stream: int, count: int, device) -> torch.Tensor:
         x = [((b >> 32) & low) ^ x[1] ^ k0, b & low, ((a >> 32) & low) ^ x[3] ^ k1, a & low]
         k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
     words = torch.stack(x, 1)
-    return torch.stack([words & 0xFFFF, words >> 16], 2).reshape(-1)[:count]
+    return torch.stack([words & 0xFFFF, words >> 16], 2).reshape(-1, 8)
+
+
+def _philox_numbers(seed: int, stream: int, count: int, device) -> torch.Tensor:
+    """``count`` 16-bit numbers as ``csrc/dropout.cu`` draws them."""
+    return _philox_blocks(seed, stream, torch.arange((count + 7) // 8, device=device)).reshape(-1)[:count]
 
 
 class _DropoutFn(torch.autograd.Function):

@@ -198,3 +198,17 @@ def test_data_parallel_replicas_draw_masks_of_their_own():
     from _mp import run_ranks
 
     run_ranks(_replica_masks, 2)
+
+
+def test_blocks_beyond_32_bits():
+    """A block's number beyond 2^32 (from 2^35 elements on) reaches the counter's second word; Python's integers."""
+    blocks = [0, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 1, 2 ** 45 + 7]
+    got = pf._philox_blocks(9, 2 ** 33 + 1, torch.tensor(blocks))
+    for block, numbers in zip(blocks, got.tolist()):
+        x, k = [block % 2 ** 32, block >> 32, 1, 2], [9, 0]
+        for _ in range(10):
+            a, b = x[0] * 0xD2511F53, x[2] * 0xCD9E8D57
+            x = [(b >> 32) ^ x[1] ^ k[0], b % 2 ** 32, (a >> 32) ^ x[3] ^ k[1], a % 2 ** 32]
+            k = [(k[0] + 0x9E3779B9) % 2 ** 32, (k[1] + 0xBB67AE85) % 2 ** 32]
+        assert numbers == [h for w in x for h in (w % 2 ** 16, w >> 16)]
+    assert len(set(map(tuple, got.tolist()))) == len(blocks)
