@@ -391,3 +391,99 @@ def test_packed_mixtral_and_tensor_parallel_on_the_gpu(form):
     for (name, a), b in zip(model.named_parameters(), exact.parameters()):
         assert off(a.grad, b.grad) < 0.04, (name, off(a.grad, b.grad))
     _lib.check_device_errors()
+
+
+def _pipelined_gradients(pipe, stages, ids, target, lengths, loss_fn, device, n_mb):
+    """Gradients of one packed step of ``pipe``, and of ``stages`` run one after the other: pairs by stage and name."""
+    pipe.optimizer, pipe.tied = None, None
+    pipe.flat.zero_grad()
+    ids, target, lengths = ids.to(device), target.to(device), lengths.to(device)
+    pipe.train_step(ids if pipe.holds_first else None, target if pipe.holds_last else None, lengths)
+    pipe.flat.fold_autograd_grads()
+    for rows, labels, counts in zip(ids.tensor_split(n_mb), target.tensor_split(n_mb), lengths.tensor_split(n_mb)):
+        h = (rows,)
+        for part in stages:
+            h = part(*h, lengths=counts)
+            h = h if isinstance(h, tuple) else (h,)
+        loss_fn(h[0], labels).backward()
+    for st in pipe.stages:
+        for (name, p), q in zip(st.submod.named_parameters(), stages[st.stage_index].parameters()):
+            yield f"{st.stage_index}.{name}", p.main_grad, q.grad
+
+
+def _llama_pipeline(device, schedule, world, dtype, dim=32, seq=S):
+    from pippy_b200.models.llama import LlamaConfig, build_llama_stage, causal_lm_loss
+    from pippy_b200.train import build_llama_pipeline
+
+    cfg = LlamaConfig.tiny(vocab_size=64, dim=dim, n_layers=4, n_heads=dim // 8 if dim < 128 else dim // 64, ffn_dim=48)
+    v = 1 if schedule == "1f1b" else 2
+    pipe = build_llama_pipeline(cfg, 4, seq, 2, device, schedule=schedule, virtual_stages=v, dtype=dtype, weight_decay=0.0)
+    stages = []
+    for s in range(v * world):
+        torch.manual_seed(s)
+        stages.append(build_llama_stage(cfg, s, v * world, device=device, dtype=dtype, pp_size=world, seq_len=seq))
+    return pipe, stages, causal_lm_loss
+
+
+def _gpt2_pipeline(device, schedule, world, dtype, dim=32, seq=S):
+    from pippy_b200.models.gpt2 import GPT2Config, build_gpt2_stage, gpt2_loss
+    from pippy_b200.train import build_gpt2_pipeline
+
+    cfg = GPT2Config(vocab_size=60, n_positions=seq, dim=dim, n_layers=4, n_heads=dim // 16 if dim < 128 else dim // 64,
+                     vocab_multiple=8)
+    v = 1 if schedule == "1f1b" else 2
+    pipe = build_gpt2_pipeline(cfg, 4, seq, 2, device, schedule=schedule, virtual_stages=v, dtype=dtype, weight_decay=0.0)
+    stages = []
+    for s in range(v * world):
+        torch.manual_seed(s)
+        stages.append(build_gpt2_stage(cfg, s, v * world, device=device, dtype=dtype))
+    if len(stages) > 1 and not (pipe.holds_first and pipe.holds_last):
+        with torch.no_grad():  # the embedding's values, as the pipeline's broadcast sets them; a gradient of its own
+            stages[-1].lm_head.weight.copy_(stages[0].wte.weight)
+    elif len(stages) > 1:
+        stages[-1].lm_head.weight = stages[0].wte.weight
+    return pipe, stages, gpt2_loss(cfg)
+
+
+FAMILIES = {"llama": _llama_pipeline, "gpt2": _gpt2_pipeline}
+
+
+def _gradients(rank, world, family, schedule):
+    pipe, stages, loss_fn = FAMILIES[family](torch.device("cpu"), schedule, world, torch.float64)
+    lengths = torch.tensor(LENGTHS + [[2, 2, 0, 12]])
+    ids = torch.randint(0, 60, (4, S), generator=torch.Generator().manual_seed(1))
+    target = torch.where(torch.cat([_inside(LENGTHS), torch.ones(1, S, dtype=torch.bool)]), ids.roll(-1, 1), -100)
+    compared = 0
+    for name, got, want in _pipelined_gradients(pipe, stages, ids, target, lengths, loss_fn, "cpu", 2):
+        # fp32 inside the plain norms and the loss, and in the buffers: 2^-24 of sums of some tens of terms
+        assert want.any() and torch.allclose(got.double(), want, rtol=1e-4, atol=1e-6), name
+        compared += 1
+    assert compared
+
+
+@pytest.mark.parametrize("family", sorted(FAMILIES))
+@pytest.mark.parametrize("schedule", ["1f1b", "interleaved_1f1b", "zero_bubble"])
+def test_gradients_of_a_packed_step_through_a_pipeline(family, schedule):
+    """Every stage of every rank: its parameters' gradients are those of the stages run one after the other."""
+    run_ranks(_gradients, 2, family, schedule)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("family", sorted(FAMILIES))
+@pytest.mark.parametrize("schedule", ["interleaved_1f1b", "zero_bubble"])
+def test_gradients_of_a_packed_step_through_two_stages_on_the_gpu(family, schedule):
+    """The kernels, two stages of one rank, weight gradients deferred (zero bubble) or not: against the stages run one after
+    the other on the same kernels without buffers."""
+    from pippy_b200.ops import _lib
+
+    S2 = 300
+    pipe, stages, loss_fn = FAMILIES[family](torch.device("cuda"), schedule, 1, torch.bfloat16, dim=128, seq=S2)
+    lengths = torch.tensor([[100, 0, 150, 3], [128, 129, 1, 0], [300, 0, 0, 0], [64, 1, 1, 30]], dtype=torch.int32)
+    ids = torch.randint(0, 60, (4, S2), generator=torch.Generator().manual_seed(1))
+    inside = torch.tensor([[t < int(row.sum()) for t in range(S2)] for row in lengths])
+    target = torch.where(inside, ids.roll(-1, 1), -100)
+    for name, got, want in _pipelined_gradients(pipe, stages, ids, target, lengths, loss_fn, "cuda", 2):
+        # the same bf16 activations on both sides; each of the two microbatches' gradients, and their sum, rounded to bf16 on
+        # one side and added in fp32 on the other: 3 roundings of 2^-9 in the mean square, twice
+        assert want.any() and (got - want.float()).norm() <= 2 * 3 ** 0.5 * 2.0 ** -9 * want.float().norm(), name
+    _lib.check_device_errors()
