@@ -170,56 +170,56 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (lane == 0) load_tile<NCH>(sV + sv * TILE_BYTES, &tmV, &v_full[sv], hkv * D, tile.start + j * 128);
         }
         ++it;
-    }
-  } else if (warp == 1) {
-    // the whole warp walks the loops; one elected lane, the same every time, issues the MMAs and their commits
-    const uint32_t idesc_t = make_idesc_bf16(128, 128, 0, 0);
-    const uint32_t idesc_acc = make_idesc_bf16(128, D, 0, 1);
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool got = warp_wait(bar, parity, abort_flag);
-      tc_fence_after_sync();
-      return got;
-    };
-    // scores: A = resident bf16 rows in TMEM, B = streamed tile, K-major
-    auto issue_scores = [&](uint32_t dst, uint32_t a, const uint8_t* tile_b, uint64_t* full, uint64_t* last) {
-      const uint64_t bd = make_smem_desc(smem_u32(tile_b), 16, 1024);
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_ts(dst, a + kk * 8, bd + (((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4), idesc_t, kk != 0);
-        umma_commit(full);
-        if (last) umma_commit(last);
       }
-      __syncwarp();
-    };
-    while (ok && next_item()) {
-      if (!(ok = wait(res_ready, it & 1) && wait(&k_full[n % kStagesK], (n / kStagesK) & 1))) break;
-      issue_scores(tS, tQ, sK + (n % kStagesK) * TILE_BYTES, s_full, nullptr);
-      if (!(ok = wait(&v_full[n % kStagesV], (n / kStagesV) & 1))) break;
-      issue_scores(tDP, tDO, sV + (n % kStagesV) * TILE_BYTES, dp_full, nblk == 1 ? res_empty : nullptr);
-      for (int j = 0; j < nblk; ++j, ++n) {
-        const bool more = j + 1 < nblk;
-        const int m = n + 1;
-        if (more) {
-          if (!(ok = wait(&k_full[m % kStagesK], (m / kStagesK) & 1) && wait(s_read, n & 1))) break;
-          issue_scores(tS, tQ, sK + (m % kStagesK) * TILE_BYTES, s_full, nullptr);
-          // what the next scores need is waited for while there is nothing to issue anyway
-          if (!(ok = wait(&v_full[m % kStagesV], (m / kStagesV) & 1))) break;
-        }
-        if (!(ok = wait(ds_ready, n & 1))) break;
-        const uint64_t kd = make_smem_desc(smem_u32(sK + (n % kStagesK) * TILE_BYTES), kChunkBytes, 1024);
+    } else if (warp == 1) {
+      // the whole warp walks the loops; one elected lane, the same every time, issues the MMAs and their commits
+      const uint32_t idesc_t = make_idesc_bf16(128, 128, 0, 0);
+      const uint32_t idesc_acc = make_idesc_bf16(128, D, 0, 1);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool got = warp_wait(bar, parity, abort_flag);
+        tc_fence_after_sync();
+        return got;
+      };
+      // scores: A = resident bf16 rows in TMEM, B = streamed tile, K-major
+      auto issue_scores = [&](uint32_t dst, uint32_t a, const uint8_t* tile_b, uint64_t* full, uint64_t* last) {
+        const uint64_t bd = make_smem_desc(smem_u32(tile_b), 16, 1024);
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)  // 16 keys a step: their dS sits in 8 columns at (kk / 4) * 64 + (kk % 4) * 8
-            umma_ts(tAcc, tDP + (kk >> 2) * 64 + (kk & 3) * 8, kd + ((kk * 2048) >> 4), idesc_acc, (j | kk) != 0);
-          umma_commit(&k_empty[n % kStagesK]);
-          if (!more) umma_commit(acc_full);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_ts(dst, a + kk * 8, bd + (((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4), idesc_t, kk != 0);
+          umma_commit(full);
+          if (last) umma_commit(last);
         }
         __syncwarp();
-        if (more)
-          issue_scores(tDP, tDO, sV + (m % kStagesV) * TILE_BYTES, dp_full, j + 2 == nblk ? res_empty : nullptr);
-      }
-      ++it;
+      };
+      while (ok && next_item()) {
+        if (!(ok = wait(res_ready, it & 1) && wait(&k_full[n % kStagesK], (n / kStagesK) & 1))) break;
+        issue_scores(tS, tQ, sK + (n % kStagesK) * TILE_BYTES, s_full, nullptr);
+        if (!(ok = wait(&v_full[n % kStagesV], (n / kStagesV) & 1))) break;
+        issue_scores(tDP, tDO, sV + (n % kStagesV) * TILE_BYTES, dp_full, nblk == 1 ? res_empty : nullptr);
+        for (int j = 0; j < nblk; ++j, ++n) {
+          const bool more = j + 1 < nblk;
+          const int m = n + 1;
+          if (more) {
+            if (!(ok = wait(&k_full[m % kStagesK], (m / kStagesK) & 1) && wait(s_read, n & 1))) break;
+            issue_scores(tS, tQ, sK + (m % kStagesK) * TILE_BYTES, s_full, nullptr);
+            // what the next scores need is waited for while there is nothing to issue anyway
+            if (!(ok = wait(&v_full[m % kStagesV], (m / kStagesV) & 1))) break;
+          }
+          if (!(ok = wait(ds_ready, n & 1))) break;
+          const uint64_t kd = make_smem_desc(smem_u32(sK + (n % kStagesK) * TILE_BYTES), kChunkBytes, 1024);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)  // 16 keys a step: their dS sits in 8 columns at (kk / 4) * 64 + (kk % 4) * 8
+              umma_ts(tAcc, tDP + (kk >> 2) * 64 + (kk & 3) * 8, kd + ((kk * 2048) >> 4), idesc_acc, (j | kk) != 0);
+            umma_commit(&k_empty[n % kStagesK]);
+            if (!more) umma_commit(acc_full);
+          }
+          __syncwarp();
+          if (more)
+            issue_scores(tDP, tDO, sV + (m % kStagesV) * TILE_BYTES, dp_full, j + 2 == nblk ? res_empty : nullptr);
+        }
+        ++it;
     }
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the k_raw barriers
@@ -511,63 +511,63 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (++blk == w.tiles) blk = w.first, ++head;
         }
         ++it;
-    }
-  } else if (warp == 1) {
-    const uint32_t idesc_t = make_idesc_bf16(128, 128, 0, 0);
-    const uint32_t idesc_acc = make_idesc_bf16(128, D, 0, 1);
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool got = warp_wait(bar, parity, abort_flag);
-      tc_fence_after_sync();
-      return got;
-    };
-    auto issue_scores = [&](uint32_t dst, const uint8_t* tile_a, const uint8_t* tile_b, uint64_t* full, uint64_t* last) {
-      const uint64_t ad = make_smem_desc(smem_u32(tile_a), 16, 1024);
-      const uint64_t bd = make_smem_desc(smem_u32(tile_b), 16, 1024);
-      if (elect_one()) {
+      }
+    } else if (warp == 1) {
+      const uint32_t idesc_t = make_idesc_bf16(128, 128, 0, 0);
+      const uint32_t idesc_acc = make_idesc_bf16(128, D, 0, 1);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool got = warp_wait(bar, parity, abort_flag);
+        tc_fence_after_sync();
+        return got;
+      };
+      auto issue_scores = [&](uint32_t dst, const uint8_t* tile_a, const uint8_t* tile_b, uint64_t* full, uint64_t* last) {
+        const uint64_t ad = make_smem_desc(smem_u32(tile_a), 16, 1024);
+        const uint64_t bd = make_smem_desc(smem_u32(tile_b), 16, 1024);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4;
-          umma_ss<1>(dst, ad + off, bd + off, idesc_t, kk != 0);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4;
+            umma_ss<1>(dst, ad + off, bd + off, idesc_t, kk != 0);
+          }
+          umma_commit(full);
+          if (last) umma_commit(last);
         }
-        umma_commit(full);
-        if (last) umma_commit(last);
-      }
-      __syncwarp();
-    };
-    // accumulation: A = P^T or dS^T (bf16 in TMEM: 16 queries in 8 columns), B = streamed tile, MN-major
-    auto issue_acc = [&](uint32_t dst, uint32_t a, const uint8_t* tile_b, int b, uint64_t* empty, uint64_t* last) {
-      const uint64_t bd = make_smem_desc(smem_u32(tile_b), kChunkBytes, 1024);
-      if (elect_one()) {
+        __syncwarp();
+      };
+      // accumulation: A = P^T or dS^T (bf16 in TMEM: 16 queries in 8 columns), B = streamed tile, MN-major
+      auto issue_acc = [&](uint32_t dst, uint32_t a, const uint8_t* tile_b, int b, uint64_t* empty, uint64_t* last) {
+        const uint64_t bd = make_smem_desc(smem_u32(tile_b), kChunkBytes, 1024);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts(dst, a + (kk >> 2) * 64 + (kk & 3) * 8, bd + ((kk * 2048) >> 4), idesc_acc, (b | kk) != 0);
-        umma_commit(empty);
-        if (last) umma_commit(last);
-      }
-      __syncwarp();
-    };
-    while (ok && next_item()) {
-      const int blocks = w.blocks;
-      if (!(ok = wait(k_full, it & 1) && wait(&q_full[n % kStagesQ], (n / kStagesQ) & 1))) break;
-      issue_scores(tS, sK, sQ + (n % kStagesQ) * TILE_BYTES, s_full, blocks == 1 ? k_empty : nullptr);
-      if (!(ok = wait(v_full, it & 1) && wait(&do_full[n % kStagesDO], (n / kStagesDO) & 1))) break;
-      issue_scores(tDP, sV, sDO + (n % kStagesDO) * TILE_BYTES, dp_full, nullptr);
-      for (int b = 0; b < blocks; ++b, ++n) {
-        const bool more = b + 1 < blocks;
-        const int m = n + 1;
-        // what the next scores need is waited for while there is nothing to issue anyway
-        if (more && !(ok = wait(&q_full[m % kStagesQ], (m / kStagesQ) & 1))) break;
-        if (!(ok = wait(p_ready, n & 1))) break;
-        issue_acc(tDV, tS, sDO + (n % kStagesDO) * TILE_BYTES, b, &do_empty[n % kStagesDO], nullptr);
-        if (more) {
-          issue_scores(tS, sK, sQ + (m % kStagesQ) * TILE_BYTES, s_full, b + 2 == blocks ? k_empty : nullptr);
-          if (!(ok = wait(&do_full[m % kStagesDO], (m / kStagesDO) & 1))) break;
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ts(dst, a + (kk >> 2) * 64 + (kk & 3) * 8, bd + ((kk * 2048) >> 4), idesc_acc, (b | kk) != 0);
+          umma_commit(empty);
+          if (last) umma_commit(last);
         }
-        if (!(ok = wait(ds_ready, n & 1))) break;
-        issue_acc(tDK, tDP, sQ + (n % kStagesQ) * TILE_BYTES, b, &q_empty[n % kStagesQ], more ? nullptr : acc_full);
-        if (more) issue_scores(tDP, sV, sDO + (m % kStagesDO) * TILE_BYTES, dp_full, nullptr);
-      }
-      ++it;
+        __syncwarp();
+      };
+      while (ok && next_item()) {
+        const int blocks = w.blocks;
+        if (!(ok = wait(k_full, it & 1) && wait(&q_full[n % kStagesQ], (n / kStagesQ) & 1))) break;
+        issue_scores(tS, sK, sQ + (n % kStagesQ) * TILE_BYTES, s_full, blocks == 1 ? k_empty : nullptr);
+        if (!(ok = wait(v_full, it & 1) && wait(&do_full[n % kStagesDO], (n / kStagesDO) & 1))) break;
+        issue_scores(tDP, sV, sDO + (n % kStagesDO) * TILE_BYTES, dp_full, nullptr);
+        for (int b = 0; b < blocks; ++b, ++n) {
+          const bool more = b + 1 < blocks;
+          const int m = n + 1;
+          // what the next scores need is waited for while there is nothing to issue anyway
+          if (more && !(ok = wait(&q_full[m % kStagesQ], (m / kStagesQ) & 1))) break;
+          if (!(ok = wait(p_ready, n & 1))) break;
+          issue_acc(tDV, tS, sDO + (n % kStagesDO) * TILE_BYTES, b, &do_empty[n % kStagesDO], nullptr);
+          if (more) {
+            issue_scores(tS, sK, sQ + (m % kStagesQ) * TILE_BYTES, s_full, b + 2 == blocks ? k_empty : nullptr);
+            if (!(ok = wait(&do_full[m % kStagesDO], (m / kStagesDO) & 1))) break;
+          }
+          if (!(ok = wait(ds_ready, n & 1))) break;
+          issue_acc(tDK, tDP, sQ + (n % kStagesQ) * TILE_BYTES, b, &q_empty[n % kStagesQ], more ? nullptr : acc_full);
+          if (more) issue_scores(tDP, sV, sDO + (m % kStagesDO) * TILE_BYTES, dp_full, nullptr);
+        }
+        ++it;
     }
   } else if (warp == 2) {
     // lse and delta of a block's queries, negative as the softmax adds them; fetched one block ahead of their buffer.  A query

@@ -188,74 +188,74 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (lane == 0)
             load_tile<NCH>(sV + s * TILE_BYTES, &tmV, w.len - key < 128 ? &v_raw[s] : &v_full[s], col, w.start + key);
         }
-    }
-  } else if (warp == 1) {
-    // the whole warp walks the loops; one elected lane, the same every time, issues the MMAs and their commits
-    const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0);
-    const uint32_t idesc_pv = make_idesc_bf16(128, D, 0, 1);
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool got = warp_wait(bar, parity, abort_flag);
-      tc_fence_after_sync();
-      return got;
-    };
-    auto issue_s = [&](int t, int stage, bool release, bool last) {
-      const uint64_t qd = make_smem_desc(smem_u32(sQ + t * TILE_BYTES), 16, 1024);
-      const uint64_t kd = make_smem_desc(smem_u32(sK + stage * TILE_BYTES), 16, 1024);
-      if (elect_one()) {
+      }
+    } else if (warp == 1) {
+      // the whole warp walks the loops; one elected lane, the same every time, issues the MMAs and their commits
+      const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0);
+      const uint32_t idesc_pv = make_idesc_bf16(128, D, 0, 1);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool got = warp_wait(bar, parity, abort_flag);
+        tc_fence_after_sync();
+        return got;
+      };
+      auto issue_s = [&](int t, int stage, bool release, bool last) {
+        const uint64_t qd = make_smem_desc(smem_u32(sQ + t * TILE_BYTES), 16, 1024);
+        const uint64_t kd = make_smem_desc(smem_u32(sK + stage * TILE_BYTES), 16, 1024);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4;
-          umma_ss<1>(tmem_base + t * 128, qd + off, kd + off, idesc_s, kk != 0);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * kChunkBytes + (kk & 3) * 32) >> 4;
+            umma_ss<1>(tmem_base + t * 128, qd + off, kd + off, idesc_s, kk != 0);
+          }
+          umma_commit(&s_full[t]);
+          if (release) umma_commit(&k_empty[stage]);
+          if (last) umma_commit(&q_empty[t]);
         }
-        umma_commit(&s_full[t]);
-        if (release) umma_commit(&k_empty[stage]);
-        if (last) umma_commit(&q_empty[t]);
-      }
-      __syncwarp();
-    };
-    auto issue_pv = [&](int t, int stage, bool first, bool release, bool last) {
-      const uint64_t vd = make_smem_desc(smem_u32(sV + stage * TILE_BYTES), kChunkBytes, 1024);
-      if (elect_one()) {
+        __syncwarp();
+      };
+      auto issue_pv = [&](int t, int stage, bool first, bool release, bool last) {
+        const uint64_t vd = make_smem_desc(smem_u32(sV + stage * TILE_BYTES), kChunkBytes, 1024);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // A = P: 16 bf16 of K per step = 8 TMEM columns
-          umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + kk * 8, vd + ((kk * 2048) >> 4), idesc_pv,
-                  !(first && kk == 0));
-        if (release) umma_commit(&v_empty[stage]);
-        if (last) umma_commit(&o_full[t]);
-      }
-      __syncwarp();
-    };
-    int done[2] = {0, 0};  // blocks so far, by tile
-    while (ok && next_item()) {
-      if (w.blocks[0] == 0) continue;
-      // stage of block j of a tile, and whether the tile is the last to read it
-      auto stage_of = [&](int t, int j) { return n + j + (w.split ? t : 0); };
-      auto last_reader = [&](int t, int j) { return w.split || t == 1 || j >= w.blocks[1]; };
-      const int nblk = max(w.blocks[0], w.blocks[1]);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (w.blocks[t] == 0 || !ok) continue;
-        const int s = stage_of(t, 0);
-        if (!(ok = wait(&q_full[t], used[t] & 1) && wait(&k_full[s & 1], (s >> 1) & 1))) continue;
-        issue_s(t, s & 1, last_reader(t, 0), w.blocks[t] == 1);
-        ++used[t];
-      }
-      for (int j = 0; ok && j < nblk; ++j) {
+          for (int kk = 0; kk < 8; ++kk)  // A = P: 16 bf16 of K per step = 8 TMEM columns
+            umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + kk * 8, vd + ((kk * 2048) >> 4), idesc_pv,
+                    !(first && kk == 0));
+          if (release) umma_commit(&v_empty[stage]);
+          if (last) umma_commit(&o_full[t]);
+        }
+        __syncwarp();
+      };
+      int done[2] = {0, 0};  // blocks so far, by tile
+      while (ok && next_item()) {
+        if (w.blocks[0] == 0) continue;
+        // stage of block j of a tile, and whether the tile is the last to read it
+        auto stage_of = [&](int t, int j) { return n + j + (w.split ? t : 0); };
+        auto last_reader = [&](int t, int j) { return w.split || t == 1 || j >= w.blocks[1]; };
+        const int nblk = max(w.blocks[0], w.blocks[1]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (j >= w.blocks[t] || !ok) continue;
-          const int s = stage_of(t, j);
-          const bool more = j + 1 < w.blocks[t];
-          // what the products need is waited for before P, which comes last
-          ok = wait(&v_full[s & 1], (s >> 1) & 1) && (!more || wait(&k_full[(s + 1) & 1], ((s + 1) >> 1) & 1)) &&
-               wait(&p_ready[t], done[t] & 1);
-          if (!ok) continue;
-          issue_pv(t, s & 1, j == 0, last_reader(t, j), !more);
-          if (more) issue_s(t, (s + 1) & 1, last_reader(t, j + 1), j + 2 == w.blocks[t]);
-          ++done[t];
+          if (w.blocks[t] == 0 || !ok) continue;
+          const int s = stage_of(t, 0);
+          if (!(ok = wait(&q_full[t], used[t] & 1) && wait(&k_full[s & 1], (s >> 1) & 1))) continue;
+          issue_s(t, s & 1, last_reader(t, 0), w.blocks[t] == 1);
+          ++used[t];
         }
-      }
-      n += w.split ? 2 : nblk;
+        for (int j = 0; ok && j < nblk; ++j) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= w.blocks[t] || !ok) continue;
+            const int s = stage_of(t, j);
+            const bool more = j + 1 < w.blocks[t];
+            // what the products need is waited for before P, which comes last
+            ok = wait(&v_full[s & 1], (s >> 1) & 1) && (!more || wait(&k_full[(s + 1) & 1], ((s + 1) >> 1) & 1)) &&
+                 wait(&p_ready[t], done[t] & 1);
+            if (!ok) continue;
+            issue_pv(t, s & 1, j == 0, last_reader(t, j), !more);
+            if (more) issue_s(t, (s + 1) & 1, last_reader(t, j + 1), j + 2 == w.blocks[t]);
+            ++done[t];
+          }
+        }
+        n += w.split ? 2 : nblk;
     }
   } else if (warp == 2) {
     uint32_t phases = 0;  // of the v_raw barriers
