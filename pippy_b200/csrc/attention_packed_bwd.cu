@@ -571,7 +571,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
   } else if (warp == 2) {
     // lse and delta of a block's queries, negative as the softmax adds them; fetched one block ahead of their buffer.  A query
-    // beyond the document gets lse = inf, so P = 2^-inf = 0 (or 2^-126, times a cleared row): no mask at a document's end.
+    // beyond the document gets lse = inf, so P = 2^-inf = 0: no mask at a document's end.
     float next[8];
     auto fetch = [&](const Item& w, int head, int blk) {
       const int row = w.start + blk * 128;

@@ -40,7 +40,10 @@ cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t s
 #ifdef __CUDACC__
 // Waits until the launches that this one was chained to are complete and their writes visible.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Called by every block, after after_previous() at the earliest, so that no launch runs ahead of the one before the last.
+// Called by every block, at its start if need be.  What keeps a launch from running ahead of the one before the last: a launch
+// that was chained itself ends after the one before it, because a thread of each of its blocks calls after_previous() at some point
+// (packed_dq_kernel only before it ends, since its memory and that of the launch before are apart); and the launch after it
+// waits for its end in after_previous().
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 #endif
 
