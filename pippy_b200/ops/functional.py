@@ -599,15 +599,13 @@ def _held_elsewhere(table: torch.Tensor, stream: int) -> bool:
     return node.metadata.pop(_MADE_ON, None) is not None
 
 
-def _graph_inputs(tables):
-    """The leaves that the op below is a function of in autograd: the tables that it writes gradients for.  Their
-    accumulation nodes are what ``backward(inputs=...)``, hooks and wrappers that count ready parameters go by.
+def _captured_inputs(tables):
+    """Under capture, the leaves that the op below is a function of in autograd.  They are the tables that it writes
+    gradients for, whose accumulation nodes ``backward(inputs=...)``, hooks and wrappers that count ready parameters go by.
 
     Such a node belongs to the stream on which the first of the graphs that hold it was made, and a backward waits for
     the streams of the nodes that it reaches.  Captured, it cannot wait for a stream outside its capture: that ends the
     process.  So a captured graph leaves a table out whose node a graph of another stream holds."""
-    if not torch.cuda.is_current_stream_capturing():
-        return tables
     stream = torch.cuda.current_stream().cuda_stream
     kept = [t for t in tables if not _held_elsewhere(t, stream)]
     return kept if len(kept) == len(tables) else kept + [_NO_STREAM]
@@ -615,14 +613,14 @@ def _graph_inputs(tables):
 
 def _note_stream(leaves) -> None:
     """After the graph of ``leaves`` is made: a node of this capture serves the capture's later embeddings too."""
-    if torch.cuda.is_current_stream_capturing():
-        for t in leaves:
-            if t is not _NO_STREAM:
-                torch.autograd.graph.get_gradient_edge(t).node.metadata[_MADE_ON] = torch.cuda.current_stream().cuda_stream
+    for t in leaves:
+        if t is not _NO_STREAM:
+            torch.autograd.graph.get_gradient_edge(t).node.metadata[_MADE_ON] = torch.cuda.current_stream().cuda_stream
 
 
 class _SortedEmbeddingFn(torch.autograd.Function):
-    """``leaves``: see :func:`_graph_inputs`.  The gradients of the tables are written by the kernels."""
+    """On the device of the tables.  ``leaves``: those that are trained, under capture see :func:`_captured_inputs`; their
+    gradients are written by the kernels."""
 
     @staticmethod
     def forward(ctx, ids, tables, positions, S: int, scale: float, *leaves):
@@ -634,14 +632,12 @@ class _SortedEmbeddingFn(torch.autograd.Function):
         if wpe is not None and (wpe.data_ptr() % 16 or not wpe.is_contiguous()):
             ptable = _aligned(wpe.detach())
         out = torch.empty(T, H, device=wte.device, dtype=wte.dtype)
-        with _on_device_of(wte):
-            _lib.check(
-                _lib.lib().pb_embed_scaled_fwd(ids.data_ptr(), table.data_ptr(), _lib.addr(ptable),
-                                               _lib.addr(positions), out.data_ptr(), T, H, S, wte.shape[0],
-                                               0 if wpe is None else wpe.shape[0], scale, _lib.err_addr(wte.device),
-                                               _lib.stream_addr()),
-                "pb_embed_scaled_fwd",
-            )
+        _lib.check(
+            _lib.lib().pb_embed_scaled_fwd(ids.data_ptr(), table.data_ptr(), _lib.addr(ptable), _lib.addr(positions),
+                                           out.data_ptr(), T, H, S, wte.shape[0], 0 if wpe is None else wpe.shape[0], scale,
+                                           _lib.err_addr(wte.device), _lib.stream_addr()),
+            "pb_embed_scaled_fwd",
+        )
         ctx.save_for_backward(ids, positions)
         wte._pb_direct_grad = True
         if wpe is not None:
@@ -662,35 +658,41 @@ class _SortedEmbeddingFn(torch.autograd.Function):
         return (None,) * len(ctx.needs_input_grad)
 
 
+def _sorted_grad_target(p):
+    """Where the kernel puts a table's gradient, and whether it writes it whole, in the table's type, or adds it in fp32."""
+    if p is None or not p.requires_grad:
+        return None, False
+    mg = getattr(p, "main_grad", None)
+    if mg is None or mg.dtype != torch.float32:
+        return torch.empty(p.shape, dtype=p.dtype, device=p.device), True
+    if mg.is_contiguous() and mg.data_ptr() % 16 == 0:
+        return mg, False
+    return torch.zeros(p.shape, dtype=torch.float32, device=p.device), False
+
+
 def _embed_sorted_wgrad(ids, positions, dout, wte, wpe, S, scale):
     T, H = dout.shape
-    # a table with an fp32 buffer has the sums added in fp32, any other gets its gradient whole, in its own type
-    added, written = {}, {}
-    for p in (wte, wpe):
-        if p is None or not p.requires_grad:
-            continue
-        mg = getattr(p, "main_grad", None)
-        if mg is None or mg.dtype != torch.float32:
-            written[p] = torch.empty(p.shape, dtype=p.dtype, device=p.device)
-        else:
-            fits = mg.is_contiguous() and mg.data_ptr() % 16 == 0
-            added[p] = mg if fits else torch.zeros(p.shape, dtype=torch.float32, device=p.device)
     lib = _lib.lib()
     with _on_device_of(dout):
-        for grads in (added, written):
-            if not grads:
-                continue
-            scratch = torch.empty(lib.pb_embed_sorted_scratch(T, H, len(grads)), dtype=torch.uint8, device=dout.device)
+        (gw, write_w), (gp, write_p) = targets = _sorted_grad_target(wte), _sorted_grad_target(wpe)
+        # one launch for both tables, unless one has an fp32 buffer and the other one has none
+        together = gw is None or gp is None or write_w == write_p
+        for a, b, write in ((gw, gp, write_w or write_p),) if together else ((gw, None, write_w), (None, gp, write_p)):
+            scratch = torch.empty(lib.pb_embed_sorted_scratch(T, H, (a is not None) + (b is not None)), dtype=torch.uint8,
+                                  device=dout.device)
             _lib.check(
-                lib.pb_embed_sorted_bwd(ids.data_ptr(), _lib.addr(positions), dout.data_ptr(), _lib.addr(grads.get(wte)),
-                                        _lib.addr(grads.get(wpe)), T, H, S, wte.shape[0], 0 if wpe is None else wpe.shape[0],
-                                        scale, int(grads is written), scratch.data_ptr(), _lib.stream_addr()),
+                lib.pb_embed_sorted_bwd(ids.data_ptr(), _lib.addr(positions), dout.data_ptr(), _lib.addr(a), _lib.addr(b), T, H, S,
+                                        wte.shape[0], 0 if wpe is None else wpe.shape[0], scale, int(write),
+                                        scratch.data_ptr(), _lib.stream_addr()),
                 "pb_embed_sorted_bwd",
             )
-        for p, g in (*added.items(), *written.items()):
-            if getattr(p, "main_grad", None) is None and p.grad is None:
+        for p, (g, _) in zip((wte, wpe), targets):
+            mg = getattr(p, "main_grad", None)
+            if g is None or g is mg:
+                continue
+            if mg is None and p.grad is None:
                 p.grad = g
-            elif g is not getattr(p, "main_grad", None):
+            else:
                 _accumulate_param_grad(p, g)
 
 
@@ -734,12 +736,12 @@ def embedding(ids, wte, wpe=None, seq_len: Optional[int] = None, scale: float = 
         if ids.dtype != torch.int64 or not ids.is_contiguous():
             ids = ids.long().contiguous()
         S = S if ids.numel() else 1
-        if not (trained and torch.is_grad_enabled()):
-            return _SortedEmbeddingFn.apply(ids, (wte, wpe), positions, S, float(scale))
         with _on_device_of(wte):
-            leaves = _graph_inputs(trained)
+            captured = torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled()
+            leaves = _captured_inputs(trained) if captured else trained
             out = _SortedEmbeddingFn.apply(ids, (wte, wpe), positions, S, float(scale), *leaves)
-            _note_stream(leaves)
+            if captured:
+                _note_stream(leaves)
         return out
     if plain:
         out = F.embedding(ids.reshape(-1), wte)
