@@ -67,8 +67,8 @@ class Dropout(nn.Module):
 
     def __init__(self, p: float):
         super().__init__()
-        if not 0.0 <= p < 1.0:
-            raise ValueError(f"dropout probability {p}")
+        if not 0.0 <= p < 1.0 - 2.0 ** -17:  # what pf.dropout takes
+            raise ValueError(f"dropout probability {p}: at least 0 and below 1 - 2^-17")
         self.p = p
 
     def forward(self, x, residual=None, seed=None, stream: int = 0):

@@ -212,3 +212,12 @@ def test_blocks_beyond_32_bits():
             k = [(k[0] + 0x9E3779B9) % 2 ** 32, (k[1] + 0xBB67AE85) % 2 ** 32]
         assert numbers == [h for w in x for h in (w % 2 ** 16, w >> 16)]
     assert len(set(map(tuple, got.tolist()))) == len(blocks)
+
+
+@pytest.mark.parametrize("p", [-0.1, 1.0 - 2.0 ** -17, 1.0, math.nan])
+def test_the_layer_refuses_what_its_forward_would(p):
+    from pippy_b200.models.layers import Dropout
+
+    with pytest.raises(ValueError):
+        Dropout(p)
+    assert Dropout(1.0 - 2.0 ** -16)(torch.ones(8), seed=1).shape == (8,)
